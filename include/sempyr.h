@@ -391,6 +391,45 @@ int sempyr_resize_crop_normalize(const uint8_t* src, int H, int W, int crop_h, i
                                  float* out01, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Token operators (no counterpart in the reference: its networks are convolutional; here they serve the generator's optional
+ * self-attention block and programs that run attention over the pyramid's feature maps or any packed token batch).
+ * Element types: SEMPYR_F32 / SEMPYR_F16 / SEMPYR_BF16; arithmetic, statistics and sums are fp32.  Strides count elements,
+ * the last dimension has stride 1.  Element counts may pass 2^31.
+ * ---------------------------------------------------------------------------------------- */
+#define SEMPYR_F32 0
+#define SEMPYR_F16 1
+#define SEMPYR_BF16 2
+
+/* y = res + keep(i) * x / (kept share), keep(i) from the counter-based generator Philox-4x32-10 (key = seed, counter = (i / 8,
+ * offset); element i takes 16-bit field i % 8, low halves first, and is kept when it lies below round((1 - p) * 65536)).
+ * rng: {seed, offset}, two int64 in DEVICE memory (a captured graph follows them).  res may be NULL.  The backward pass is the
+ * same call on the gradient without res.  Pointers need only their element's alignment. */
+int sempyr_dropout_add(int dtype, const void* x, const void* res, void* y, int64_t n, double p, const int64_t* rng, void* stream);
+
+/* Norms of queries and keys for each head and their rotary position in one pass.  x: [tokens][heads][dim] views of queries and
+ * keys (say of one fused projection), y and the gradients: contiguous.  y = R(positions) (x * rsqrt(mean(x^2) + eps) * w);
+ * weights wq / wk [dim] of both or NULL (no norm).  The first sections[0] + sections[1] + ... pairs of a head are rotated, the
+ * pairs of section k by positions[token][k] * freq; the rest of the head is not rotated.  A pair is (j, j + pairs), or (2j, 2j + 1)
+ * when interleaved.  positions: int32 [tokens][axes].  freqs: per pair round(2^64 * freq / 2 pi) (0 <= freq <= 2 pi).
+ * dim even, <= 512; axes <= 4. */
+typedef struct sempyr_rope_desc {
+    int64_t tokens;
+    int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+    int32_t dtype, heads_q, heads_k, dim;
+    int32_t axes, sections[4];
+    int32_t interleaved;
+    float eps;
+} sempyr_rope_desc;
+int sempyr_qk_norm_rope_fwd(const sempyr_rope_desc* d, const void* xq, const void* xk, const int32_t* positions,
+                            const uint64_t* freqs, const void* wq, const void* wk, void* yq, void* yk, void* stream);
+/* gq / gk: gradients of the outputs (contiguous).  dwq / dwk (with weights): [dim] in the element type, summed in a fixed order.
+ * scratch: that many floats as sempyr_qk_norm_rope_bwd_scratch says (NULL without weights). */
+int sempyr_qk_norm_rope_bwd_scratch(const sempyr_rope_desc* d, int64_t* floats);
+int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq, const void* xk, const int32_t* positions,
+                            const uint64_t* freqs, const void* wq, const void* wk, const void* gq, const void* gk,
+                            void* dq, void* dk, void* dwq, void* dwk, float* scratch, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Replay of a captured loop body (no counterpart in the reference: its loop body, train_model.py:300-349, is issued op by
  * op from Python).  sempyr_replay_create walks a captured hipGraph_t once (kernel / memset / 1-D device memcpy / empty
  * nodes and their dependency edges) and lays the DAG out on up to max_streams HIP streams; sempyr_replay_launch re-issues

@@ -17,6 +17,7 @@ MAX_PHASES = 4
 CONV_FWD, CONV_DGRAD, CONV_WGRAD = 0, 1, 2
 NORM_BATCH, NORM_INSTANCE, NORM_LAYER = 0, 1, 2
 MATH_F32, MATH_BF16X3 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH = 0, 1, 2, 3
 
 
@@ -50,6 +51,13 @@ class MaskTarget(ctypes.Structure):
 
 class AccumItem(ctypes.Structure):
     _fields_ = [("dst", c_void_p), ("src", c_void_p * 4), ("numel", ctypes.c_int64), ("assign", ctypes.c_int32)]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("q_stride_token", ctypes.c_int64), ("q_stride_head", ctypes.c_int64),
+                ("k_stride_token", ctypes.c_int64), ("k_stride_head", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32), ("dim", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("sections", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
 ADAM_MAX_TENSORS = 64
@@ -116,6 +124,10 @@ SIGNATURES = {
     "sempyr_gp_fwd_static": [_P, c_int, c_int, _P, _P, _P],
     "sempyr_gp_bwd": [_P, _P, _P, c_int, c_int, _P, _P],
     "sempyr_channel_sum": [_P, c_int, c_int, c_int, c_float, _P, c_int, _P, _P],
+    "sempyr_dropout_add": [c_int, _P, _P, _P, c_int64, ctypes.c_double, _P, _P],
+    "sempyr_qk_norm_rope_fwd": [ctypes.POINTER(RopeDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "sempyr_qk_norm_rope_bwd_scratch": [ctypes.POINTER(RopeDesc), ctypes.POINTER(c_int64)],
+    "sempyr_qk_norm_rope_bwd": [ctypes.POINTER(RopeDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "sempyr_replay_create": [_P, c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_create_on": [_P, c_int, ctypes.POINTER(c_void_p), c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_launch": [_P, _P],

@@ -7,6 +7,7 @@ expressed with differentiable Functions, so the WGAN-GP double backward
 discriminator uses.  There is no CPU path: non-CUDA(HIP) tensors raise.
 """
 import ctypes
+import fractions
 import os
 import threading
 
@@ -22,7 +23,7 @@ L = _lib.lib
 __all__ = ["conv2d", "conv_transpose2d", "norm_act", "norm_add_norm_act", "bn_eval_act", "act", "add_act", "mul", "normalize",
            "avg_pool2", "upsample2", "max_pool3s2", "global_avg_pool", "mean", "l1_mean", "gp_loss", "lerp_rows",
            "input_grads_only", "async_param_grads", "join_side_streams", "ACT_NONE", "ACT_RELU", "ACT_LRELU", "ACT_TANH", "NORM_BATCH", "NORM_INSTANCE",
-           "NORM_LAYER"]
+           "NORM_LAYER", "AxialRope", "qk_norm_rope", "dropout_add"]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -1817,3 +1818,223 @@ def lerp_rows(real, fake, alpha):
     check(L.sempyr_lerp_rows(real.data_ptr(), fake.data_ptr(), alpha.data_ptr(), out.data_ptr(), rows, real.numel() // rows,
                              _stream()), "sempyr_lerp_rows")
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# token operators: fp32, fp16 and bf16 tensors whose last dimension has stride 1; tensors of another device than the current
+# one run there.  First derivatives only (the critic, which needs second ones, has no tokens).
+# ------------------------------------------------------------------------------------------------
+_DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _token_dtype(tensors, what):
+    """The common element-type code of `tensors` (name -> tensor, None entries skipped)."""
+    dtypes = {t.dtype for t in tensors.values() if t is not None}
+    if len(dtypes) != 1 or next(iter(dtypes)) not in _DTYPE_CODE:
+        raise _lib.SempyrError(f"{what}: one type of float32, float16 or bfloat16 for all of {', '.join(tensors)} expected, got "
+                               + ", ".join(f"{n} {t.dtype}" for n, t in tensors.items() if t is not None))
+    return _DTYPE_CODE[next(iter(dtypes))]
+
+
+def _one_device(tensors, what):
+    """Refuses CPU tensors and tensors of several GPUs; returns the device."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.SempyrError(f"{what}: {name}: the sempyr operators run on the GPU only (got a {t.device} tensor); "
+                                   "there is no CPU fallback")
+        if dev is not None and t.device != dev:
+            raise _lib.SempyrError(f"{what}: tensors on {dev} and {t.device}")
+        dev = t.device
+    return dev
+
+
+class _on_device:
+    """Makes `device` current where it is not (the launches below go to the current device's current stream)."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.prev = _cur_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _rows(t):
+    """t with unit stride in the last dimension (copied only where it has another one)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _no_second_order(what, *grads):
+    if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
+        raise NotImplementedError(f"{what}: second derivatives are not available")
+
+
+class AxialRope:
+    """Rotary position of tokens that lie on one to four axes (a text; height and width of a map; time, height and width of a
+    video).  `sections[a]` pairs of a head turn with the position on axis a; pairs beyond the sections are left alone.
+
+    Pair i of an axis with n pairs turns by position * base^(-i / n); with `shared`, the axes share ONE spectrum over all
+    pairs and pair j turns by base^(-j / sum(sections)).  A pair is elements (j, j + sum(sections)), or (2j, 2j + 1) with
+    `interleaved`.  The device table is made on first use on a device; call `table(device)` before a graph capture."""
+
+    def __init__(self, sections, base=10000.0, interleaved=False, shared=False):
+        self.sections = tuple(int(n) for n in sections)
+        if not 1 <= len(self.sections) <= 4 or min(self.sections) < 0 or sum(self.sections) < 1:
+            raise _lib.SempyrError(f"AxialRope: one to four sections with at least one pair expected, got {tuple(sections)}")
+        if not float(base) >= 1.0 or float(base) == float("inf"):
+            raise _lib.SempyrError(f"AxialRope: base must be finite and at least 1, got {base}")
+        self.base, self.interleaved, self.shared = float(base), bool(interleaved), bool(shared)
+        self.pairs = sum(self.sections)
+        self._tables = {}
+
+    def frequencies(self):
+        """The angle of one position step, per pair (radians)."""
+        if self.shared:
+            return [self.base ** (-(j / self.pairs)) for j in range(self.pairs)]
+        return [self.base ** (-(i / n)) for n in self.sections for i in range(n)]
+
+    def fractions(self):
+        """frequencies() / 2 pi as 64-bit fractions of a turn (exact integer arithmetic on the fp64 frequency)."""
+        two_pi = fractions.Fraction("6.28318530717958647692528676655900576839")
+        return [int(fractions.Fraction(f) / two_pi * 2 ** 64 + fractions.Fraction(1, 2)) for f in self.frequencies()]
+
+    def table(self, device):
+        device = torch.device(device)
+        t = self._tables.get(device)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.SempyrError("AxialRope: first use on this device during a graph capture; call table(device) before it")
+            signed = [f - 2 ** 64 if f >= 2 ** 63 else f for f in self.fractions()]
+            t = self._tables[device] = torch.tensor(signed, dtype=torch.int64).to(device)
+        return t
+
+
+def _rope_desc(q, k, rope, dtype, eps):
+    sec = list(rope.sections) + [0] * (4 - len(rope.sections))
+    return _lib.RopeDesc(q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), dtype, q.shape[1], k.shape[1], q.shape[2],
+                         len(rope.sections), (ctypes.c_int32 * 4)(*sec), int(rope.interleaved), eps)
+
+
+class _QkNormRope(Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, rope, wq, wk, eps, dtype):
+        with _on_device(q.device):
+            q, k, positions = _rows(q), _rows(k), positions.contiguous()
+            if wq is not None:
+                wq, wk = wq.contiguous(), wk.contiguous()
+            yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            check(L.sempyr_qk_norm_rope_fwd(ctypes.byref(_rope_desc(q, k, rope, dtype, eps)), q.data_ptr(), k.data_ptr(),
+                                            positions.data_ptr(), rope.table(q.device).data_ptr(), _p(wq), _p(wk), yq.data_ptr(),
+                                            yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
+        ctx.save_for_backward(q, k, positions, wq, wk)
+        ctx.cfg = (rope, eps, dtype)
+        return yq, yk
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        _no_second_order("qk_norm_rope", gq, gk)
+        q, k, positions, wq, wk = ctx.saved_tensors
+        rope, eps, dtype = ctx.cfg
+        with _on_device(q.device):
+            gq, gk = gq.contiguous(), gk.contiguous()
+            dq, dk = torch.empty_like(gq), torch.empty_like(gk)
+            dwq = dwk = scratch = None
+            desc = _rope_desc(q, k, rope, dtype, eps)
+            if wq is not None:
+                n = ctypes.c_int64()
+                check(L.sempyr_qk_norm_rope_bwd_scratch(ctypes.byref(desc), ctypes.byref(n)), "sempyr_qk_norm_rope_bwd_scratch")
+                scratch = torch.empty(n.value, dtype=torch.float32, device=q.device)
+                dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+            check(L.sempyr_qk_norm_rope_bwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), positions.data_ptr(),
+                                            rope.table(q.device).data_ptr(), _p(wq), _p(wk), gq.data_ptr(), gk.data_ptr(),
+                                            dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), _p(scratch), _stream()),
+                  "sempyr_qk_norm_rope_bwd")
+        if _INPUT_GRADS_ONLY:
+            dwq = dwk = None
+        elif dwq is not None and dwq.dtype == torch.float32:
+            if _stash(wq, dwq):
+                dwq = None
+            if _stash(wk, dwk):
+                dwk = None
+        return dq, dk, None, None, dwq, dwk, None, None
+
+
+def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps=1e-6):
+    """RMS norm of every head of queries [tokens, heads_q, dim] and keys [tokens, heads_k, dim] and their rotary position, in
+    one pass: R(positions) (x / sqrt(mean(x^2) + eps) * weight).  `positions`: int32 [tokens] or [tokens, axes]; `rope`: an
+    AxialRope; weights [dim] of both or neither (then only the rotation).  q and k may be views of one projection.  Returns two
+    contiguous tensors; differentiable in q, k and the weights."""
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or 0 in q.shape[1:] or 0 in k.shape[1:]:
+        raise _lib.SempyrError(f"qk_norm_rope: [tokens, heads, dim] queries and keys of equal tokens and dim expected, got "
+                               f"{tuple(q.shape)} and {tuple(k.shape)}")
+    if positions.dim() == 1:
+        positions = positions[:, None]
+    if tuple(positions.shape) != (q.shape[0], len(rope.sections)) or positions.dtype != torch.int32:
+        raise _lib.SempyrError(f"qk_norm_rope: int32 positions [{q.shape[0]}, {len(rope.sections)}] expected, got "
+                               f"{positions.dtype} {tuple(positions.shape)}")
+    dim = q.shape[2]
+    if dim % 2 or dim > 512 or rope.pairs > dim // 2:
+        raise _lib.SempyrError(f"qk_norm_rope: an even head dim up to 512 with room for {rope.pairs} pairs expected, got {dim}")
+    if (q_weight is None) != (k_weight is None):
+        raise _lib.SempyrError("qk_norm_rope: norm weights of both or of neither")
+    for w in (q_weight, k_weight):
+        if w is not None and tuple(w.shape) != (dim,):
+            raise _lib.SempyrError(f"qk_norm_rope: weights of shape ({dim},) expected, got {tuple(w.shape)}")
+    if not 0.0 <= eps < float("inf"):
+        raise _lib.SempyrError(f"qk_norm_rope: eps must be finite and not negative, got {eps}")
+    dtype = _token_dtype({"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
+    _one_device({"q": q, "k": k, "positions": positions, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
+    return _apply(_QkNormRope, q, k, positions, rope, q_weight, k_weight, float(eps), dtype)
+
+
+def _dropout_raw(x, res, p, rng, dtype):
+    with _on_device(x.device):
+        x = x.contiguous()
+        res = res if res is None else res.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        check(L.sempyr_dropout_add(dtype, x.data_ptr(), _p(res), y.data_ptr(), x.numel(), p, rng.data_ptr(), _stream()),
+              "sempyr_dropout_add")
+    return y
+
+
+class _DropoutAdd(Function):
+    @staticmethod
+    def forward(ctx, x, res, p, rng, dtype):
+        rng = rng.contiguous()
+        ctx.save_for_backward(rng)
+        ctx.cfg = (p, dtype, res is not None)
+        return _dropout_raw(x, res, p, rng, dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        _no_second_order("dropout_add", g)
+        p, dtype, has_res = ctx.cfg
+        gx = _dropout_raw(g, None, p, ctx.saved_tensors[0], dtype) if ctx.needs_input_grad[0] else None
+        return gx, (g if has_res else None), None, None, None
+
+
+def dropout_add(x, res, p, rng):
+    """res + dropout(x, p) (res None: the dropout alone); the keep decisions are never stored, forward and backward compute them
+    from `rng`, an int64 tensor {seed, offset} on the device (fresh values for every call: a captured graph reads what the tensor
+    holds at replay; the tensor must not change before the backward pass has run).  An element is dropped with the probability
+    p rounded to a multiple of 2^-16, kept ones are scaled by the reciprocal of the exact keep probability."""
+    if res is not None and x.shape != res.shape:
+        raise _lib.SempyrError(f"dropout_add: x {tuple(x.shape)} and res {tuple(res.shape)} differ")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise _lib.SempyrError(f"dropout_add: p must lie in [0, 1], got {p}")
+    if rng.dtype != torch.int64 or rng.numel() != 2:
+        raise _lib.SempyrError("dropout_add: rng must be an int64 tensor {seed, offset}")
+    dtype = _token_dtype({"x": x, "res": res}, "dropout_add")
+    _one_device({"x": x, "res": res, "rng": rng}, "dropout_add")
+    return _apply(_DropoutAdd, x, res, p, rng, dtype)

@@ -1,0 +1,95 @@
+"""Token operators without a GPU: refusals, the frequency table, the generator's published test vectors, C entry checks."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from token_oracle import dropout_gain, frequencies, philox4x32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from semantic_pyramid_for_image_generation_amd import ops
+    return ops
+
+
+def test_philox_known_answers():
+    """The generator's published vectors (counter, key -> words) hold for the oracle the GPU results are compared with."""
+    assert philox4x32((0, 0, 0, 0), (0, 0)) == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+    m = 0xFFFFFFFF
+    assert philox4x32((m, m, m, m), (m, m)) == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+    g = dropout_gain(4096, 0.25, 5, 7)
+    assert abs(float(g.mean()) - 1.0) < 5 * math.sqrt(0.25 / 0.75 / 4096)
+
+
+@pytest.mark.parametrize("sections,shared", [((8,), False), ((16, 24, 24), True), ((5, 0, 3), False), ((13, 14), False)])
+def test_rope_fractions(ops, sections, shared):
+    rope = ops.AxialRope(sections, 10000.0, shared=shared)
+    want = frequencies(sections, 10000.0, shared)
+    assert rope.frequencies() == want
+    for f, turn in zip(want, rope.fractions()):
+        assert abs(turn / 2 ** 64 - f / (2 * math.pi)) <= 2.0 ** -52
+        for pos in (0, 1, -1, 123456, -(2 ** 31), 2 ** 31 - 1):         # the wrapping product is the angle modulo one turn
+            wrapped = (turn * pos) % 2 ** 64 / 2 ** 64
+            assert abs(math.cos(2 * math.pi * wrapped) - math.cos(pos * f)) <= 2.0 ** -52 * max(1, abs(pos)) * 8
+
+
+def test_rope_refusals(ops):
+    E = ops._lib.SempyrError
+    for bad in ((), (0,), (-1, 4), (1,) * 5):
+        with pytest.raises(E):
+            ops.AxialRope(bad)
+    for base in (0.5, float("inf"), float("nan")):
+        with pytest.raises(E):
+            ops.AxialRope((4,), base)
+    rope = ops.AxialRope((4, 4))
+    q, k = torch.zeros(3, 2, 16), torch.zeros(3, 1, 16)
+    pos = torch.zeros(3, 2, dtype=torch.int32)
+    w = torch.ones(16)
+    for args in ((q[0], k, pos, rope), (q, k[:2], pos, rope), (q, k[..., :8], pos, rope), (q[:, :0], k, pos, rope),
+                 (q, k, pos[:2], rope), (q, k, pos.long(), rope), (q, k, pos[:, :1], rope), (q, k, pos[:, 0], rope),
+                 (q[..., :15], k[..., :15], pos, rope), (q[..., :14], k[..., :14], pos, rope),
+                 (q, k, pos, rope, w), (q, k, pos, rope, w[:8], w), (q, k, pos, rope, w, w, -1.0),
+                 (q, k, pos, rope, w, w, float("nan")), (q, k.half(), pos, rope), (q.double(), k.double(), pos, rope),
+                 (q, k, pos, rope, w.half(), w.half())):
+        with pytest.raises(E):
+            ops.qk_norm_rope(*args)
+    with pytest.raises(E, match="GPU only"):
+        ops.qk_norm_rope(q, k, pos, rope, w, w)
+
+
+def test_dropout_refusals(ops):
+    E = ops._lib.SempyrError
+    x, rng = torch.zeros(4, 4), torch.zeros(2, dtype=torch.int64)
+    for args in ((x, x[:2], 0.1, rng), (x, None, -0.1, rng), (x, None, 1.1, rng), (x, None, float("nan"), rng),
+                 (x, None, 0.1, rng[:1]), (x, None, 0.1, rng.int()), (x, x.half(), 0.1, rng), (x.double(), None, 0.1, rng)):
+        with pytest.raises(E):
+            ops.dropout_add(*args)
+    with pytest.raises(E, match="GPU only"):
+        ops.dropout_add(x, None, 0.1, rng)
+
+
+def test_c_entries_refuse_bad_descriptors():
+    """Every refusal happens on the host, before a launch."""
+    from semantic_pyramid_for_image_generation_amd import _lib
+    L = _lib.lib
+    sec = lambda *s: (ctypes.c_int32 * 4)(*s)
+    good = dict(tokens=4, q_stride_token=32, q_stride_head=16, k_stride_token=16, k_stride_head=16, dtype=_lib.F32, heads_q=2,
+                heads_k=1, dim=16, axes=1, sections=sec(8), interleaved=0, eps=1e-6)
+    for change in (dict(dim=15), dict(dim=514), dict(dtype=3), dict(heads_q=0), dict(axes=0), dict(axes=5), dict(sections=sec(9)),
+                   dict(sections=sec(0)), dict(sections=sec(-1)), dict(tokens=-1), dict(eps=-1.0), dict(eps=float("nan"))):
+        d = _lib.RopeDesc(**{**good, **change})
+        assert L.sempyr_qk_norm_rope_fwd(ctypes.byref(d), 16, 16, 16, 16, 16, 16, 16, 16, 0) < 0, change
+        assert L.sempyr_last_error_string()
+        assert L.sempyr_qk_norm_rope_bwd(ctypes.byref(d), *[16] * 13, 0) < 0, change
+    d = _lib.RopeDesc(**good)
+    assert L.sempyr_qk_norm_rope_fwd(ctypes.byref(d), 0, 16, 16, 16, 16, 16, 16, 16, 0) < 0        # null queries
+    assert L.sempyr_qk_norm_rope_fwd(ctypes.byref(d), 16, 16, 16, 16, 16, 0, 16, 16, 0) < 0        # one weight only
+    assert L.sempyr_qk_norm_rope_fwd(None, 16, 16, 16, 16, 16, 16, 16, 16, 0) < 0
+    n = ctypes.c_int64()
+    assert L.sempyr_qk_norm_rope_bwd_scratch(ctypes.byref(d), ctypes.byref(n)) == 0 and n.value >= 2 * 16
+    for args in ((7, 16, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, -1, 0.1, 16), (0, 16, 0, 16, 8, 1.5, 16), (0, 16, 0, 16, 8, -0.5, 16),
+                 (0, 0, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, 8, 0.1, 0), (0, 16, 0, 16, 8, float("nan"), 16)):
+        assert L.sempyr_dropout_add(*args, 0) < 0, args
+    assert L.sempyr_dropout_add(0, 0, 0, 0, 0, 0.1, 0, 0) == 0             # nothing to do
