@@ -429,6 +429,28 @@ int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq, const voi
                             const uint64_t* freqs, const void* wq, const void* wk, const void* gq, const void* gk,
                             void* dq, void* dk, void* dwq, void* dwk, float* scratch, void* stream);
 
+/* Attention over packed sequences: o = softmax(scale q k^T + mask) v for every sequence s and query head h, whose keys are
+ * head h / (heads_q / heads_k).  q / o: [total_q][heads_q][dim], k / v: [total_k][heads_k][dim] (token and head strides of the
+ * inputs in the descriptor; o and the gradients contiguous).  Sequence s: queries cu_q[s] .. cu_q[s + 1] - 1, keys cu_k[s] ..
+ * cu_k[s + 1] - 1, of which the first len_k[s] count (len_k NULL: all; a cache slot may be longer than what it holds).  All
+ * tables are int32 in DEVICE memory; entry 0 counts as 0, entries are clamped to the tensors.  causal: query i of a sequence
+ * with lq queries and lk keys sees keys 0 .. i + lk - lq.  Rows that see no key, and rows of q / k behind the last sequence,
+ * give zeros.  lse (optional): [heads_q][total_q] floats for the backward pass.  dim <= 128 and, like all strides and pointers,
+ * whole 16-byte vectors; token strides up to 2^23 elements. */
+typedef struct sempyr_attention_desc {
+    int64_t total_q, total_k;
+    int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    int32_t dtype, heads_q, heads_k, dim;
+    int32_t nseq, causal;
+    float scale;
+} sempyr_attention_desc;
+int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
+                         const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, void* stream);
+/* go: gradient of o (contiguous); delta: heads_q * total_q floats of workspace.  No atomics: the sums have a fixed order. */
+int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const void* o,
+                         const float* lse, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,
+                         void* dq, void* dk, void* dv, float* delta, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Replay of a captured loop body (no counterpart in the reference: its loop body, train_model.py:300-349, is issued op by
  * op from Python).  sempyr_replay_create walks a captured hipGraph_t once (kernel / memset / 1-D device memcpy / empty

@@ -60,6 +60,14 @@ class RopeDesc(ctypes.Structure):
                 ("sections", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64), ("q_stride_token", ctypes.c_int64),
+                ("q_stride_head", ctypes.c_int64), ("k_stride_token", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
+                ("v_stride_token", ctypes.c_int64), ("v_stride_head", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32), ("dim", ctypes.c_int32), ("nseq", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 ADAM_MAX_TENSORS = 64
 CONCAT_MAX = 8
 LINCOMB_MAX = 6
@@ -128,6 +136,8 @@ SIGNATURES = {
     "sempyr_qk_norm_rope_fwd": [ctypes.POINTER(RopeDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "sempyr_qk_norm_rope_bwd_scratch": [ctypes.POINTER(RopeDesc), ctypes.POINTER(c_int64)],
     "sempyr_qk_norm_rope_bwd": [ctypes.POINTER(RopeDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "sempyr_attention_fwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "sempyr_attention_bwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "sempyr_replay_create": [_P, c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_create_on": [_P, c_int, ctypes.POINTER(c_void_p), c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_launch": [_P, _P],

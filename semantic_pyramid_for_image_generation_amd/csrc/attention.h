@@ -1,0 +1,17 @@
+// Launchers of the packed attention (one file each) and what they share with the C entries in attention.hip.
+#pragma once
+#include "attn_tile.h"
+
+namespace attn {
+
+// Dynamic LDS above 64 KiB has to be asked for, per kernel and device (a host-side attribute, fine under stream capture).
+static inline int allow_lds(const void* kernel, int bytes) {
+    if (bytes <= 65536) return 0;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) { sempyr_set_error("attention: %d bytes of LDS: %s", bytes, hipGetErrorString(e)); return (int)e; }
+    return 0;
+}
+
+int launch_fwd(int dtype, const Params& p, hipStream_t st);
+int launch_bwd(int dtype, const Params& p, float* delta, hipStream_t st);
+}

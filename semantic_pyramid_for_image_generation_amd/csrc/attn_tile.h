@@ -1,0 +1,249 @@
+// Tiles of the attention kernels (attention_fwd.hip, attention_bwd.hip, attention_split.hip) on gfx950.
+//
+// Matrix products run on the 32x32 MFMA shapes with the ROWS OF THE RESULT in a lane's registers and one COLUMN per lane pair
+// (l, l + 32): register i of lane l holds row 8 (i / 4) + 4 (l / 32) + i % 4 of column l % 32.  Scores are computed transposed
+// (keys are rows, a query is a column), so a query's softmax runs over a lane's own registers plus one exchange between the
+// lane halves, and the probabilities are, as they lie in the registers, the right operand of the next product: a sum over k
+// may run in any order as long as both operands agree, and the order used everywhere is
+//     element j of lane half h in the t-th group of 16 = row 16 t + 8 (j / 4) + 4 h + j % 4.
+// No probability goes through LDS.
+//
+// A tile in LDS is [rows][CH chunks of 16 bytes]; chunk c of row r lies at c ^ swz(r).  That spreads both ways of reading over
+// the banks: "row fragments" (lane = row, 8 consecutive elements) and "column fragments" (lane = column, 8 rows in the order
+// above; 16-bit types by the transposing ds_read_b64_tr_b16, which hands 16 lanes a 4 x 16 block by columns).
+// Tiles are filled by LDS DMA (buffer_load_dwordx4 ... lds), which writes a wave's 64 x 16 bytes in lane order: the permutation
+// is applied to the addresses that are read.  The buffer descriptor ends with the last valid row, so rows behind a sequence
+// and columns behind the head arrive as zeros and nothing outside is ever touched.
+#pragma once
+#include "tokens.h"
+
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+#define LDS_PTR __attribute__((address_space(3)))
+
+struct Params {
+    const void *q, *k, *v;                                   // [rows][heads][dim], strides in elements
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    void* o;                                                 // contiguous [total_q][heads_q][dim]
+    float* lse;                                              // [heads_q][total_q]: log2 of a row's sum of exponentials, or null
+    const void* go;                                          // backward: gradient of o, contiguous
+    const float* delta;                                      // backward: [heads_q][total_q] rowsum(go * o)
+    void *dq, *dk, *dv;                                      // backward: contiguous
+    const int32_t *cu_q, *cu_k, *len_k;
+    int total_q, total_k, nseq, heads_q, heads_k, group, dim, causal;
+    float scale, scale_log2;                                 // scale * log2(e)
+};
+
+// ---------------------------------------------------------------------------------------------- element types
+template <typename T> struct Elem;
+template <> struct Elem<bf16> {
+    typedef bf16 Frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<f16> {
+    typedef f16 Frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<float> {
+    typedef float Frag __attribute__((ext_vector_type(8)));
+    // the group of 16 in eight steps of two (lane half h of step i holds its element i)
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// registers 8 t .. 8 t + 7 of a result as the right operand of the next product.  16-bit types round here: probabilities and
+// score gradients enter the matrix pipe in the inputs' type, their sums stay fp32.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Frag frag_of(const f32x16& s, int t) {
+    typename Elem<T>::Frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)s[t * 8 + j];
+    return f;
+}
+
+// ---------------------------------------------------------------------------------------------- tiles
+template <typename T, int DPAD, int ROWS>
+struct Tile {
+    typedef typename Elem<T>::Frag Frag;
+    static constexpr int SZ = sizeof(T), ROWB = DPAD * SZ, CH = ROWB / 16, BYTES = ROWS * ROWB;
+    static constexpr int LOADS = BYTES / 1024;               // 1 KiB DMA instructions of a tile
+    static_assert(CH >= 4 && (CH & (CH - 1)) == 0 && BYTES % 1024 == 0, "tile shape");
+
+    static __device__ __forceinline__ int swz(int r) {
+        return CH >= 16 ? (r & 3) << 2 | (r >> 2 & 3) : CH == 8 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : r >> 2 & 3;
+    }
+    // byte offset of a lane's row fragment in row block 0, group 0; see row()
+    static __device__ __forceinline__ int row_base(int lane) {
+        const int r = lane & 31, h = lane >> 5;
+        return r * ROWB + (((SZ == 2 ? h : 2 * h) ^ swz(r)) << 4);
+    }
+    // elements 16 slab + 8 h .. + 8 of row 32 block + lane % 32
+    static __device__ __forceinline__ Frag row(const char* tile, int base, int block, int slab) {
+        const char* p = tile + block * 32 * ROWB;
+        if constexpr (SZ == 2) return *reinterpret_cast<const Frag*>(p + (base ^ slab * 32));
+        else {
+            typedef float f4 __attribute__((ext_vector_type(4)));
+            const f4 a = *reinterpret_cast<const f4*>(p + (base ^ slab * 64)), b = *reinterpret_cast<const f4*>(p + (base ^ slab * 64 ^ 16));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    static __device__ __forceinline__ int col_base(int lane) {
+        const int h = lane >> 5;
+        if (SZ == 2) {
+            const int r4 = (lane & 15) >> 2, r = h * 4 + r4, c = (lane >> 4 & 1) * 2 + ((lane & 3) >> 1);
+            return r * ROWB + ((c ^ swz(r)) << 4) + (lane & 1) * 8;
+        }
+        return h * 4 * ROWB + (((lane & 31) >> 2 ^ swz(h * 4)) << 4) + (lane & 3) * 4;
+    }
+    // column 32 block + lane % 32, rows 16 t + 8 (j / 4) + 4 h + j % 4
+    static __device__ __forceinline__ Frag col(const char* tile, int base, int block, int t) {
+        Frag f;
+        if constexpr (SZ == 2) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const char* p = tile + (t * 16 + u * 8) * ROWB + (base ^ block * 64 ^ u * 32);
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR s16x4*)(p));
+                typedef T V4 __attribute__((ext_vector_type(4)));
+                const V4 y = __builtin_bit_cast(V4, x);      // (as a whole: the cast of one vector element takes element 0)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[u * 4 + j] = y[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = (j / 4) * 8 + j % 4;
+                f[j] = *reinterpret_cast<const float*>(tile + (t * 16 + r) * ROWB + (base ^ block * 128 ^ swz(r) << 4));
+            }
+        }
+        return f;
+    }
+};
+
+// Fills tiles from rows of a strided tensor.  `waves` waves share a tile; a lane's source offsets are fixed.
+template <typename T, int DPAD, int ROWS, int WAVES>
+struct Filler {
+    typedef Tile<T, DPAD, ROWS> Tl;
+    static constexpr int N = Tl::LOADS / WAVES;              // instructions a wave issues
+    static_assert(Tl::LOADS % WAVES == 0, "whole instructions per wave");
+    int voff[N];
+    int stride_bytes, row_bytes, wave;
+
+    __device__ __forceinline__ void init(int64_t stride_elems, int dim, int wave_, int lane) {
+        stride_bytes = (int)stride_elems * Tl::SZ;           // the host has checked that 64 rows stay below 2^31 bytes
+        row_bytes = dim * Tl::SZ;
+        wave = wave_;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int p = (j * WAVES + wave) * 64 + lane, r = p / Tl::CH, c = (p % Tl::CH) ^ Tl::swz(r);
+            voff[j] = c * 16 < row_bytes ? r * stride_bytes + c * 16 : (int)0x80000000;      // behind every buffer's end: zeros
+        }
+    }
+    // rows 0 .. ROWS - 1 from `base` (a wave-uniform address); rows from `valid` on become zeros
+    __device__ __forceinline__ void issue(const void* base, int valid, char* tile) const {
+        const int rows = valid < ROWS ? valid : ROWS;
+        const int bytes = rows > 0 ? (rows - 1) * stride_bytes + row_bytes : 0;
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LDS_PTR void*)(tile + (j * WAVES + wave) * 1024), 16, voff[j], 0, 0, 0);
+    }
+};
+
+// waits until at most N of this wave's vector memory accesses are in flight
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// 8 consecutive elements of each group of 16 of a global row, in row-fragment order (zeros for an absent row, behind the head)
+template <typename T, int DPAD>
+__device__ __forceinline__ void load_row_frags(typename Elem<T>::Frag* f, const T* row, bool present, int dim, int lane) {
+    const int h = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < DPAD / 16; ++s) {
+        const int d = s * 16 + h * 8;
+        if constexpr (sizeof(T) == 2) {
+            typename Elem<T>::Frag z = {};
+            f[s] = present && d < dim ? *reinterpret_cast<const typename Elem<T>::Frag*>(row + d) : z;
+        } else {
+            typedef float f4 __attribute__((ext_vector_type(4)));
+            const f4 z = {0.f, 0.f, 0.f, 0.f};
+            const f4 a = present && d < dim ? *reinterpret_cast<const f4*>(row + d) : z;
+            const f4 b = present && d + 4 < dim ? *reinterpret_cast<const f4*>(row + d + 4) : z;
+            f[s] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+}
+
+// 4 consecutive elements
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    typedef T V __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<V*>(p) = V{(T)a, (T)b, (T)c, (T)d};
+}
+
+// ---------------------------------------------------------------------------------------------- packed sequences
+// Sequence s covers rows cu[s] .. cu[s + 1] - 1; the first entry counts as 0, rows behind the last entry form one more,
+// key-less sequence (their results are zeros).  Every entry is clamped to the tensor, so a bad table reads nothing outside.
+__device__ __forceinline__ int row_bound(const int32_t* cu, int s, int nseq, int total) {
+    if (s <= 0) return 0;
+    if (s > nseq) return total;
+    const int v = cu[s];
+    return v < 0 ? 0 : v > total ? total : v;
+}
+
+struct Seq { int q0, lq, k0, lk, kcap; };       // first rows, queries, keys that count, rows of the key slot
+
+__device__ __forceinline__ Seq seq_of(const Params& p, int s) {
+    Seq q;
+    q.q0 = row_bound(p.cu_q, s, p.nseq, p.total_q);
+    q.lq = row_bound(p.cu_q, s + 1, p.nseq, p.total_q) - q.q0;
+    q.k0 = row_bound(p.cu_k, s, p.nseq, p.total_k);
+    q.kcap = row_bound(p.cu_k, s + 1, p.nseq, p.total_k) - q.k0;
+    if (q.lq < 0) q.lq = 0;
+    if (q.kcap < 0) q.kcap = 0;
+    q.lk = q.kcap;
+    if (s >= p.nseq) q.lk = 0;
+    else if (p.len_k) { const int n = p.len_k[s]; q.lk = n < 0 ? 0 : n < q.kcap ? n : q.kcap; }
+    return q;
+}
+
+// Tiles of R rows are numbered so that sequence s owns slots cu[s] / R + s .. (at least as many as it has tiles; the rest are
+// empty): no table has to be built and lengths may change between replays of a captured graph.  The search probes 64
+// entries at a time.
+__device__ __forceinline__ int find_seq(const int32_t* cu, int nseq, int total, int slot, int R, int lane) {
+    int lo = 0, hi = nseq;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64, c = lo + (lane + 1) * step;
+        const bool ok = c <= hi && row_bound(cu, c, nseq, total) / R + c <= slot;
+        lo += __popcll(__ballot(ok)) * step;
+        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+    }
+    return lo;
+}
+__host__ __device__ inline int num_slots(int nseq, int total, int R) { return total / R + nseq + 1; }
+
+// Workgroup -> (slot, kv head, head in group).  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets
+// whole kv heads where there are enough, else every X-th slot of one, so that K and V of a head are read into few L2s; within
+// an XCD the heads of a group come next to each other, and late slots (the long rows of a causal mask) come first.
+struct Work { int slot, kvh, g; };
+__host__ __device__ inline int xcd_classes(int heads_k) { return heads_k % 8 == 0 ? 8 : heads_k % 4 == 0 ? 4 : heads_k % 2 == 0 ? 2 : 1; }
+static inline int64_t work_blocks(int slots, int heads_k, int inner) {
+    const int g = xcd_classes(heads_k), x = 8 / g;
+    return 8ll * ((slots + x - 1) / x) * (heads_k / g) * inner;
+}
+__device__ __forceinline__ Work work_of(int block, int slots, int heads_k, int inner) {
+    const int cls = xcd_classes(heads_k), x = 8 / cls, per = heads_k / cls;
+    const int xcd = block & 7, j = block >> 3;
+    Work w;
+    w.g = j % inner;
+    w.kvh = xcd % cls + cls * (j / inner % per);
+    w.slot = slots - 1 - (j / inner / per * x + xcd / cls);
+    return w;
+}
+
+}  // namespace attn

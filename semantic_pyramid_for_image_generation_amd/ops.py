@@ -23,7 +23,7 @@ L = _lib.lib
 __all__ = ["conv2d", "conv_transpose2d", "norm_act", "norm_add_norm_act", "bn_eval_act", "act", "add_act", "mul", "normalize",
            "avg_pool2", "upsample2", "max_pool3s2", "global_avg_pool", "mean", "l1_mean", "gp_loss", "lerp_rows",
            "input_grads_only", "async_param_grads", "join_side_streams", "ACT_NONE", "ACT_RELU", "ACT_LRELU", "ACT_TANH", "NORM_BATCH", "NORM_INSTANCE",
-           "NORM_LAYER", "AxialRope", "qk_norm_rope", "dropout_add"]
+           "NORM_LAYER", "AxialRope", "qk_norm_rope", "attention", "dropout_add"]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -1995,6 +1995,91 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps=1e-6):
     dtype = _token_dtype({"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
     _one_device({"q": q, "k": k, "positions": positions, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
     return _apply(_QkNormRope, q, k, positions, rope, q_weight, k_weight, float(eps), dtype)
+
+
+def _attn_rows(t):
+    """t as the kernels read it: unit stride in the last dimension, rows on 16 bytes, token stride at least a row (an expanded
+    dimension has none) and below 2^23 elements; anything else is copied."""
+    unit = 16 // t.element_size()
+    st, sh, sd = t.stride()
+    if sd != 1 or st % unit or sh % unit or t.data_ptr() % 16 or st < t.shape[2] or st > 2 ** 23:
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t
+
+
+def _attn_desc(q, k, v, nseq, causal, scale, dtype):
+    return _lib.AttentionDesc(q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                              dtype, q.shape[1], k.shape[1], q.shape[2], nseq, causal, scale)
+
+
+class _Attention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, len_k, causal, scale, dtype):
+        with _on_device(q.device):
+            q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+            cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+            len_k = len_k if len_k is None else len_k.contiguous()
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad[:3]) else None
+            check(L.sempyr_attention_fwd(ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype)), q.data_ptr(),
+                                         k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k), o.data_ptr(),
+                                         _p(lse), _stream()), "sempyr_attention_fwd")
+        if lse is not None:
+            ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, len_k)
+            ctx.cfg = (causal, scale, dtype)
+        return o
+
+    @staticmethod
+    def backward(ctx, g):
+        _no_second_order("attention", g)
+        q, k, v, o, lse, cu_q, cu_k, len_k = ctx.saved_tensors
+        causal, scale, dtype = ctx.cfg
+        with _on_device(q.device):
+            g = g.contiguous()
+            g = g if g.data_ptr() % 16 == 0 else g.clone()
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            delta = torch.empty_like(lse)
+            check(L.sempyr_attention_bwd(ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype)), q.data_ptr(),
+                                         k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
+                                         cu_k.data_ptr(), _p(len_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                         delta.data_ptr(), _stream()), "sempyr_attention_bwd")
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
+    """softmax(scale q k^T + mask) v over packed sequences: q [total_q, heads_q, dim], k / v [total_k, heads_k, dim] with heads_q
+    a multiple of heads_k (consecutive query heads share a key head).  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys
+    cu_k[s] .. cu_k[s + 1] - 1 (cu_k None: cu_q), of which the first len_k[s] count (None: all); int32 tensors on the device,
+    the first entry of a table is 0.  causal: the last query sees all keys, the one before it one less, and so on.  Queries
+    that see no key give zeros, as do rows behind the last sequence; keys that nobody sees get zero gradients, and what lies
+    in rows behind len_k[s] is never read.  scale None: dim ** -0.5.  dim: a multiple of 8 (fp32: 4) up to 128.
+    Differentiable in q, k and v; the sums of both passes have a fixed order."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2] or 0 in q.shape[1:] or 0 in k.shape[1:] or \
+            q.shape[1] % k.shape[1]:
+        raise _lib.SempyrError("attention: q [total_q, heads_q, dim] and k, v [total_k, heads_k, dim] with heads_q a multiple of "
+                               f"heads_k expected, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    dtype = _token_dtype({"q": q, "k": k, "v": v}, "attention")
+    unit = 16 // q.element_size()
+    if q.shape[2] % unit or q.shape[2] > 128:
+        raise _lib.SempyrError(f"attention: a head dim that is a multiple of {unit}, at most 128, expected, got {q.shape[2]}")
+    if max(q.shape[0], k.shape[0]) > 0x7FFFFF00:
+        raise _lib.SempyrError("attention: more than 2^31 rows")
+    if cu_k is None:
+        if q.shape[0] != k.shape[0]:
+            raise _lib.SempyrError("attention: cu_k is needed where queries and keys differ in number")
+        cu_k = cu_q
+    for name, t in (("cu_q", cu_q), ("cu_k", cu_k), ("len_k", len_k)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != cu_q.numel() - (name == "len_k") or cu_q.numel() < 1:
+            raise _lib.SempyrError(f"attention: {name}: int32 entries, one for each of the {cu_q.numel() - 1} sequences"
+                                   f"{'' if name == 'len_k' else ' and one more'}, expected, got {t.dtype} {tuple(t.shape)}")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise _lib.SempyrError(f"attention: scale must be positive and finite, got {scale}")
+    _one_device({"q": q, "k": k, "v": v, "cu_q": cu_q, "cu_k": cu_k, "len_k": len_k}, "attention")
+    return _apply(_Attention, q, k, v, cu_q, cu_k, len_k, bool(causal), scale, dtype)
 
 
 def _dropout_raw(x, res, p, rng, dtype):

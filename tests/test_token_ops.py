@@ -70,6 +70,42 @@ def test_dropout_refusals(ops):
         ops.dropout_add(x, None, 0.1, rng)
 
 
+def test_attention_refusals(ops):
+    E = ops._lib.SempyrError
+    q, k = torch.zeros(6, 4, 16), torch.zeros(6, 2, 16)
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32)
+    for args in ((q[0], k, k, cu), (q, k, k[:5], cu), (q, k[..., :8], k[..., :8], cu), (q[:, :3], k, k, cu), (q[:, :0], k, k, cu),
+                 (q, k.half(), k, cu), (q.double(), k.double(), k.double(), cu), (q[..., :6], k[..., :6], k[..., :6], cu),
+                 (torch.zeros(6, 1, 132),) * 3 + (cu,), (torch.zeros(6, 1, 12, dtype=torch.half),) * 3 + (cu,), (q[:5], k, k, cu),
+                 (q, k, k, cu.long()), (q, k, k, cu[None]), (q, k, k, cu[:0]), (q, k, k, cu, cu[:2]), (q, k, k, cu, cu, cu),
+                 (q, k, k, cu, cu, None, True, 0.0), (q, k, k, cu, cu, None, True, -1.0), (q, k, k, cu, cu, None, True, float("inf")),
+                 (q, k, k, cu, cu, None, True, float("nan"))):
+        with pytest.raises(E):
+            ops.attention(*args)
+    with pytest.raises(E, match="GPU only"):
+        ops.attention(q, k, k, cu, causal=True)
+
+
+def test_attention_oracle_gradients():
+    """The oracle's gradients are those of differentiating its definition."""
+    import token_oracle
+    gen = torch.Generator().manual_seed(0)
+    q, k, v, g = (torch.randn(n, h, 8, generator=gen, dtype=torch.float64).float() for n, h in ((11, 4), (15, 2), (15, 2), (11, 4)))
+    seqs = [(0, 4, 0, 3), (4, 7, 3, 9)]
+    got = token_oracle.attention(q, k, v, g, seqs, True, 0.4)
+    leaves = [t.double().requires_grad_() for t in (q, k, v)]
+    out = torch.zeros(11, 4, 8, dtype=torch.float64)
+    for q0, lq, k0, lk in seqs:
+        for h in range(4):
+            s = 0.4 * leaves[0][q0:q0 + lq, h] @ leaves[1][k0:k0 + lk, h // 2].t()
+            hide = torch.arange(lk)[None] > torch.arange(lq)[:, None] + lk - lq
+            e = torch.where(hide, torch.zeros_like(s), s.exp())
+            out[q0:q0 + lq, h] = e @ leaves[2][k0:k0 + lk, h // 2] / e.sum(-1, keepdim=True).clamp_min(1e-30)
+    grads = torch.autograd.grad(out, leaves, g.double())
+    for (w, e), t in zip(got, [out.detach(), *grads]):
+        assert torch.allclose(w, t, rtol=0, atol=1e-12)
+
+
 def test_c_entries_refuse_bad_descriptors():
     """Every refusal happens on the host, before a launch."""
     from semantic_pyramid_for_image_generation_amd import _lib
@@ -93,3 +129,26 @@ def test_c_entries_refuse_bad_descriptors():
                  (0, 0, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, 8, 0.1, 0), (0, 16, 0, 16, 8, float("nan"), 16)):
         assert L.sempyr_dropout_add(*args, 0) < 0, args
     assert L.sempyr_dropout_add(0, 0, 0, 0, 0, 0.1, 0, 0) == 0             # nothing to do
+
+
+def test_attention_c_entries_refuse():
+    from semantic_pyramid_for_image_generation_amd import _lib
+    L = _lib.lib
+    good = dict(total_q=8, total_k=8, q_stride_token=64, q_stride_head=16, k_stride_token=32, k_stride_head=16, v_stride_token=32,
+                v_stride_head=16, dtype=_lib.F32, heads_q=4, heads_k=2, dim=16, nseq=1, causal=1, scale=0.25)
+    for change in (dict(dim=0), dict(dim=6), dict(dim=132), dict(dtype=-1), dict(heads_q=3), dict(heads_k=0), dict(nseq=-1),
+                   dict(scale=0.0), dict(scale=float("nan")), dict(total_q=-1), dict(total_k=2 ** 31), dict(k_stride_token=33),
+                   dict(k_stride_token=8), dict(v_stride_token=2 ** 24), dict(q_stride_head=-16)):
+        d = _lib.AttentionDesc(**{**good, **change})
+        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9) < 0, change
+        assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 14) < 0, change
+    d = _lib.AttentionDesc(**good)
+    for hole in range(7):
+        if hole == 5:
+            continue                                    # len_k may be absent
+        args = [16] * 9
+        args[hole] = 0
+        assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0, hole
+    args = [16] * 9
+    args[1] = 20                                        # keys that are not 16-byte aligned
+    assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0

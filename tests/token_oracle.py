@@ -83,3 +83,60 @@ def dropout_gain(n, p, seed, offset):
             fields += [word & 0xFFFF, word >> 16]
     f = torch.tensor(fields[:n], dtype=torch.int64)
     return (f < t).double() * (65536.0 / t if t else 0.0)
+
+
+def attention(q, k, v, g, seqs, causal, scale):
+    """(o, dq, dk, dv), each with its error bound, of packed sequences; seqs: (first query, queries, first key, keys).
+
+    u = U, h = half a step of the type.  A score is a sum of dim products: off by dim u sum|q||k|; the exponent's fma, the row
+    maximum and the exponential add a few u of its size, so a probability is off by eps_p relative, and by h once it is rounded
+    for the second product (fp16: by 2^-25 absolute where it is subnormal).  Sums over n terms add n u of the absolute sum."""
+    h = half_step(q.dtype)
+    sub = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    if q.dtype == torch.float32:
+        h = U
+    group = q.shape[1] // k.shape[1]
+    dim = q.shape[2]
+    q, k, v, g = (t.double() for t in (q, k, v, g))
+    out = [torch.zeros_like(t) for t in (q, q, k, v)]
+    err = [torch.zeros_like(t) for t in (q, q, k, v)]
+    for q0, lq, k0, lk in seqs:
+        if lq == 0 or lk == 0:
+            continue
+        for hd in range(q.shape[1]):
+            kh = hd // group
+            Q, G, K, V = q[q0:q0 + lq, hd], g[q0:q0 + lq, hd], k[k0:k0 + lk, kh], v[k0:k0 + lk, kh]
+            S = scale * Q @ K.t()
+            seen = torch.ones(lq, lk, dtype=torch.bool)
+            if causal:
+                seen = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + (lk - lq)
+            S = S.masked_fill(~seen, float("-inf"))
+            P = torch.softmax(S, dim=-1).nan_to_num(0.0)
+            P = torch.where(seen, P, torch.zeros_like(P))
+            size = torch.where(seen, S, torch.zeros_like(S)).abs().amax(dim=-1, keepdim=True)
+            eps_p = scale * dim * U * (Q.abs() @ K.abs().t()).amax(dim=-1, keepdim=True) + 8 * U * (1 + 1.5 * size)
+            n = lk + lk // 16 + 16
+            o = P @ V
+            PV = P @ V.abs()
+            eo = (2 * eps_p + h + 2 * n * U) * PV + (2 * n * U + 2 * h) * o.abs() + sub * V.abs().sum(dim=0)
+            dP = G @ V.t()
+            delta = (G * o).sum(dim=-1, keepdim=True)
+            dS = P * (dP - delta)
+            e_dp = dim * U * (G.abs() @ V.abs().t())
+            e_de = (G.abs() * eo).sum(dim=-1, keepdim=True) + dim * U * (G * o).abs().sum(dim=-1, keepdim=True)
+            e_p = 2 * eps_p + 2 * n * U
+            e_ds = P * (e_dp + e_de) + dS.abs() * (e_p + 4 * U + h) + sub * seen
+            e_pv = P * (e_p + h) + sub * seen
+            m = lq * group + 16
+            out[0][q0:q0 + lq, hd] = o
+            err[0][q0:q0 + lq, hd] = eo
+            out[1][q0:q0 + lq, hd] = scale * dS @ K
+            err[1][q0:q0 + lq, hd] = scale * (e_ds @ K.abs() + n * U * dS.abs() @ K.abs()) + 2 * h * out[1][q0:q0 + lq, hd].abs()
+            out[2][k0:k0 + lk, kh] += scale * dS.t() @ Q
+            err[2][k0:k0 + lk, kh] += scale * (e_ds.t() @ Q.abs() + m * U * dS.t().abs() @ Q.abs())
+            out[3][k0:k0 + lk, kh] += P.t() @ G
+            err[3][k0:k0 + lk, kh] += e_pv.t() @ G.abs() + m * U * P.t() @ G.abs()
+    err[2] += 2 * h * out[2].abs()
+    err[3] += 2 * h * out[3].abs()
+    # what no formula covers: results next to the smallest numbers of the type
+    return [(o, e + 1e-37 + sub) for o, e in zip(out, err)]
