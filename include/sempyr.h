@@ -444,8 +444,12 @@ typedef struct sempyr_attention_desc {
     int32_t nseq, causal;
     float scale;
 } sempyr_attention_desc;
+/* Few rows (single new tokens, small maps) are computed with the keys split over workgroups, which takes a workspace: that many
+ * floats as sempyr_attention_workspace says (often 0), used by this call only until it has run. */
+int sempyr_attention_workspace(const sempyr_attention_desc* d, int64_t* floats);
 int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
-                         const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, void* stream);
+                         const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, float* workspace,
+                         int64_t workspace_size, void* stream);
 /* go: gradient of o (contiguous); delta: heads_q * total_q floats of workspace.  No atomics: the sums have a fixed order. */
 int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const void* o,
                          const float* lse, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,

@@ -30,8 +30,22 @@ int fill_params(const sempyr_attention_desc* d, attn::Params& p, const char* who
 
 }  // namespace
 
+static int64_t workspace_floats(const attn::Params& p, const attn::SplitPlan& plan) {
+    return plan.splits > 1 ? (int64_t)plan.splits * p.total_q * p.heads_q * (p.dim + 2) : 0;
+}
+
+extern "C" int sempyr_attention_workspace(const sempyr_attention_desc* d, int64_t* floats)
+{
+    attn::Params p;
+    if (int rc = fill_params(d, p, "attention_workspace")) return rc;
+    if (!floats) SEMPYR_FAIL("attention_workspace: null pointer");
+    *floats = workspace_floats(p, attn::plan_split(d->dtype, p));
+    return 0;
+}
+
 extern "C" int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
-                                    const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, void* stream)
+                                    const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, float* workspace,
+                                    int64_t workspace_size, void* stream)
 {
     attn::Params p;
     if (int rc = fill_params(d, p, "attention_fwd")) return rc;
@@ -39,7 +53,12 @@ extern "C" int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* 
     if (!q || !o || (p.total_k > 0 && (!k || !v)) || !cu_q || !cu_k) SEMPYR_FAIL("attention_fwd: null pointer");
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) SEMPYR_FAIL("attention_fwd: tensors must be 16-byte aligned");
     p.q = q; p.k = k; p.v = v; p.cu_q = cu_q; p.cu_k = cu_k; p.len_k = len_k; p.o = o; p.lse = lse;
-    return attn::launch_fwd(d->dtype, p, (hipStream_t)stream);
+    const attn::SplitPlan plan = attn::plan_split(d->dtype, p);
+    if (plan.splits == 0) return attn::launch_fwd(d->dtype, p, (hipStream_t)stream);
+    const int64_t need = workspace_floats(p, plan);
+    if (need > 0 && (!workspace || workspace_size < need || !aligned16(workspace)))
+        SEMPYR_FAIL("attention_fwd: %lld floats of 16-byte aligned workspace expected, got %lld", (long long)need, (long long)workspace_size);
+    return attn::launch_split(d->dtype, p, plan, workspace, (hipStream_t)stream);
 }
 
 extern "C" int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const void* o,

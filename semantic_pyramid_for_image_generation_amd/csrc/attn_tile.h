@@ -157,7 +157,9 @@ struct Filler {
 // waits until at most N of this wave's vector memory accesses are in flight
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
+// waits until this wave's LDS reads have returned: a buffer may be refilled only after that
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // 8 consecutive elements of each group of 16 of a global row, in row-fragment order (zeros for an absent row, behind the head)
 template <typename T, int DPAD>

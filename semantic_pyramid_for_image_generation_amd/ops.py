@@ -2022,9 +2022,12 @@ class _Attention(Function):
             len_k = len_k if len_k is None else len_k.contiguous()
             o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
             lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad[:3]) else None
-            check(L.sempyr_attention_fwd(ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype)), q.data_ptr(),
-                                         k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k), o.data_ptr(),
-                                         _p(lse), _stream()), "sempyr_attention_fwd")
+            desc = ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype))
+            n = ctypes.c_int64()
+            check(L.sempyr_attention_workspace(desc, ctypes.byref(n)), "sempyr_attention_workspace")
+            ws = _workspace(4 * n.value, q.device)
+            check(L.sempyr_attention_fwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k),
+                                         o.data_ptr(), _p(lse), _p(ws), n.value, _stream()), "sempyr_attention_fwd")
         if lse is not None:
             ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, len_k)
             ctx.cfg = (causal, scale, dtype)

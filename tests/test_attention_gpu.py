@@ -39,6 +39,10 @@ CASES = {
     "slots": ([1, 1, 3], [96, 96, 96], [17, 0, 96], 0, 10, 2, 64, True),             # cache slots, partly used
     "no_keys": ([4, 5], [0, 0], [0, 0], 0, 2, 2, 16, False),
     "group": ([70], [190], [190], 0, 40, 1, 16, True),
+    "token": ([1, 1, 1, 1], [700, 700, 700, 700], [700, 1, 0, 333], 0, 8, 1, 128, True),     # new tokens, split keys
+    "tokens_many_heads": ([2, 1], [150, 40], [150, 33], 2, 70, 1, 48, True),                 # a group wider than a tile
+    "many": ([140] * 10 + [3], [140] * 10 + [3], [140] * 10 + [3], 0, 28, 4, 32, True),      # enough tiles for the one-pass kernel
+    "many_full": ([300, 290, 1], [300, 290, 77], [300, 290, 70], 5, 64, 64, 16, False),
     "heads8": ([150, 20], [150, 20], [150, 20], 0, 16, 8, 24, True),
 }
 

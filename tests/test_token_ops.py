@@ -140,15 +140,20 @@ def test_attention_c_entries_refuse():
                    dict(scale=0.0), dict(scale=float("nan")), dict(total_q=-1), dict(total_k=2 ** 31), dict(k_stride_token=33),
                    dict(k_stride_token=8), dict(v_stride_token=2 ** 24), dict(q_stride_head=-16)):
         d = _lib.AttentionDesc(**{**good, **change})
-        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9) < 0, change
+        n = ctypes.c_int64()
+        assert L.sempyr_attention_workspace(ctypes.byref(d), ctypes.byref(n)) < 0, change
+        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, 0, 16) < 0, change
         assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 14) < 0, change
     d = _lib.AttentionDesc(**good)
-    for hole in range(7):
-        if hole == 5:
-            continue                                    # len_k may be absent
-        args = [16] * 9
+    for hole in (0, 1, 2, 3, 4, 6):                     # (5: len_k may be absent)
+        args = [16] * 9 + [0, 16]
         args[hole] = 0
         assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0, hole
-    args = [16] * 9
+    args = [16] * 9 + [0, 16]
     args[1] = 20                                        # keys that are not 16-byte aligned
     assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0
+    n = ctypes.c_int64()
+    d = _lib.AttentionDesc(**{**good, "total_q": 1, "total_k": 4096})
+    assert L.sempyr_attention_workspace(ctypes.byref(d), ctypes.byref(n)) == 0 and n.value > 0
+    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, n.value - 1, 16) < 0 and b"workspace" in L.sempyr_last_error_string()
+    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 8, 0, n.value, 16) < 0
