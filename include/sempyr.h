@@ -435,7 +435,8 @@ int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq, const voi
  * cu_k[s + 1] - 1, of which the first len_k[s] count (len_k NULL: all; a cache slot may be longer than what it holds).  All
  * tables are int32 in DEVICE memory; entry 0 counts as 0, entries are clamped to the tensors.  causal: query i of a sequence
  * with lq queries and lk keys sees keys 0 .. i + lk - lq.  Rows that see no key, and rows of q / k behind the last sequence,
- * give zeros.  lse (optional): [heads_q][total_q] floats for the backward pass.  dim <= 128 and, like all strides and pointers,
+ * give zeros.  For the backward pass: stats (optional), [heads_q][total_q] floats, twice as many for fp32; o_low (optional, 16-bit types), a second
+ * tensor like o that takes what rounding o left, so that the gradients do not carry o's rounding.  dim <= 128 and, like all strides and pointers,
  * whole 16-byte vectors; token strides up to 2^23 elements. */
 typedef struct sempyr_attention_desc {
     int64_t total_q, total_k;
@@ -448,11 +449,11 @@ typedef struct sempyr_attention_desc {
  * floats as sempyr_attention_workspace says (often 0), used by this call only until it has run. */
 int sempyr_attention_workspace(const sempyr_attention_desc* d, int64_t* floats);
 int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
-                         const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, float* workspace,
+                         const int32_t* cu_k, const int32_t* len_k, void* o, void* o_low, float* stats, float* workspace,
                          int64_t workspace_size, void* stream);
 /* go: gradient of o (contiguous); delta: heads_q * total_q floats of workspace.  No atomics: the sums have a fixed order. */
 int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const void* o,
-                         const float* lse, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,
+                         const void* o_low, const float* stats, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,
                          void* dq, void* dk, void* dv, float* delta, void* stream);
 
 /* ------------------------------------------------------------------------------------------

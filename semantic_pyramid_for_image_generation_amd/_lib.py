@@ -137,8 +137,8 @@ SIGNATURES = {
     "sempyr_qk_norm_rope_bwd_scratch": [ctypes.POINTER(RopeDesc), ctypes.POINTER(c_int64)],
     "sempyr_qk_norm_rope_bwd": [ctypes.POINTER(RopeDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "sempyr_attention_workspace": [ctypes.POINTER(AttentionDesc), ctypes.POINTER(c_int64)],
-    "sempyr_attention_fwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P],
-    "sempyr_attention_bwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "sempyr_attention_fwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P],
+    "sempyr_attention_bwd": [ctypes.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "sempyr_replay_create": [_P, c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_create_on": [_P, c_int, ctypes.POINTER(c_void_p), c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int32)],
     "sempyr_replay_launch": [_P, _P],

@@ -14,7 +14,7 @@ static inline int allow_lds(const void* kernel, int bytes) {
 
 // Few rows: query heads and queries packed into a tile's 32 columns, keys split (splits 0: the one-pass kernel is taken).
 struct SplitPlan { int head_chunks, heads, queries, splits; };
-SplitPlan plan_split(int dtype, const Params& p);
+SplitPlan plan_split(const Params& p);
 int launch_split(int dtype, const Params& p, const SplitPlan& plan, float* ws, hipStream_t st);
 
 int launch_fwd(int dtype, const Params& p, hipStream_t st);

@@ -39,21 +39,21 @@ extern "C" int sempyr_attention_workspace(const sempyr_attention_desc* d, int64_
     attn::Params p;
     if (int rc = fill_params(d, p, "attention_workspace")) return rc;
     if (!floats) SEMPYR_FAIL("attention_workspace: null pointer");
-    *floats = workspace_floats(p, attn::plan_split(d->dtype, p));
+    *floats = workspace_floats(p, attn::plan_split(p));
     return 0;
 }
 
 extern "C" int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const int32_t* cu_q,
-                                    const int32_t* cu_k, const int32_t* len_k, void* o, float* lse, float* workspace,
+                                    const int32_t* cu_k, const int32_t* len_k, void* o, void* o_low, float* stats, float* workspace,
                                     int64_t workspace_size, void* stream)
 {
     attn::Params p;
     if (int rc = fill_params(d, p, "attention_fwd")) return rc;
     if (p.total_q == 0) return 0;
     if (!q || !o || (p.total_k > 0 && (!k || !v)) || !cu_q || !cu_k) SEMPYR_FAIL("attention_fwd: null pointer");
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)) SEMPYR_FAIL("attention_fwd: tensors must be 16-byte aligned");
-    p.q = q; p.k = k; p.v = v; p.cu_q = cu_q; p.cu_k = cu_k; p.len_k = len_k; p.o = o; p.lse = lse;
-    const attn::SplitPlan plan = attn::plan_split(d->dtype, p);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(o_low)) SEMPYR_FAIL("attention_fwd: tensors must be 16-byte aligned");
+    p.q = q; p.k = k; p.v = v; p.cu_q = cu_q; p.cu_k = cu_k; p.len_k = len_k; p.o = o; p.o_low = o_low; p.stats = stats;
+    const attn::SplitPlan plan = attn::plan_split(p);
     if (plan.splits == 0) return attn::launch_fwd(d->dtype, p, (hipStream_t)stream);
     const int64_t need = workspace_floats(p, plan);
     if (need > 0 && (!workspace || workspace_size < need || !aligned16(workspace)))
@@ -62,19 +62,19 @@ extern "C" int sempyr_attention_fwd(const sempyr_attention_desc* d, const void* 
 }
 
 extern "C" int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* q, const void* k, const void* v, const void* o,
-                                    const float* lse, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,
+                                    const void* o_low, const float* stats, const void* go, const int32_t* cu_q, const int32_t* cu_k, const int32_t* len_k,
                                     void* dq, void* dk, void* dv, float* delta, void* stream)
 {
     attn::Params p;
     if (int rc = fill_params(d, p, "attention_bwd")) return rc;
     if (p.total_q == 0 && p.total_k == 0) return 0;
-    if ((p.total_q > 0 && (!q || !o || !lse || !go || !dq || !delta)) || (p.total_k > 0 && (!k || !v || !dk || !dv)) || !cu_q || !cu_k)
+    if ((p.total_q > 0 && (!q || !o || !stats || !go || !dq || !delta)) || (p.total_k > 0 && (!k || !v || !dk || !dv)) || !cu_q || !cu_k)
         SEMPYR_FAIL("attention_bwd: null pointer");
-    const void* ptrs[] = {q, k, v, o, go, dq, dk, dv};
+    const void* ptrs[] = {q, k, v, o, o_low, go, dq, dk, dv};
     for (const void* x : ptrs)
         if (!aligned16(x)) SEMPYR_FAIL("attention_bwd: tensors must be 16-byte aligned");
     if ((int64_t)d->heads_q * d->dim > (int64_t)1 << 23) SEMPYR_FAIL("attention_bwd: rows of more than 2^23 elements");
     p.q = q; p.k = k; p.v = v; p.cu_q = cu_q; p.cu_k = cu_k; p.len_k = len_k;
-    p.o = const_cast<void*>(o); p.lse = const_cast<float*>(lse); p.go = go; p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
+    p.o = const_cast<void*>(o); p.o_low = const_cast<void*>(o_low); p.stats = const_cast<float*>(stats); p.go = go; p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
     return attn::launch_bwd(d->dtype, p, delta, (hipStream_t)stream);
 }

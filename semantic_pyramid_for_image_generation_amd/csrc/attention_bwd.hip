@@ -1,7 +1,7 @@
-// Backward of the packed attention.  With P = exp2(c S - lse) recomputed from the forward's row statistics:
+// Backward of the packed attention.  With P recomputed from the forward's row statistics (see Stats):
 //     dV = P^T dO,  dP = dO V^T,  dS = P o (dP - delta),  delta = rowsum(dO o O),  dQ = scale dS K,  dK = scale dS^T Q
-// Two kernels without atomics, each owning what it sums, so the result does not depend on timing: one workgroup per 128 keys
-// walks over the queries of all heads of its group (dK, dV), one per 128 queries walks over the keys (dQ).  That costs seven
+// Two kernels without atomics, each owning what it sums, so the result does not depend on timing: one workgroup per 32 or 64
+// keys walks over the queries of all heads of its group (dK, dV), one per 128 queries walks over the keys (dQ).  That costs seven
 // products a tile pair instead of five; the two that are repeated are what the order of an atomic sum would otherwise cost.
 #include "attn_tile.h"
 #include "attention.h"
@@ -10,9 +10,11 @@ namespace attn {
 
 constexpr int BM = 128, BN = 64;
 
-// delta[head][row] = sum over d of go * o, 16 lanes a row
+// delta[head][row] = sum over d of go * o, 16 lanes a row.  For 16-bit types o is taken with what its rounding left (o_low):
+// an error of delta is common to a row, so dQ would carry the rounding of o (2^-9 for bf16) in full.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restrict__ go, const T* __restrict__ o, float* __restrict__ delta,
+__global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restrict__ go, const T* __restrict__ o, const T* __restrict__ o_low,
+                                                              float* __restrict__ delta,
                                                               int64_t rows, int total_q, int heads, int dim)
 {
     constexpr int N = Vec16<T>::N;
@@ -23,6 +25,12 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restric
         float a[N], b[N];
         load_floats<T, N>(go + row * dim + d, a);
         load_floats<T, N>(o + row * dim + d, b);
+        if (o_low) {
+            float c[N];
+            load_floats<T, N>(o_low + row * dim + d, c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) b[i] += c[i];
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) sum = fmaf(a[i], b[i], sum);
     }
@@ -31,113 +39,169 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restric
     if (threadIdx.x % 16 == 0) delta[(row % heads) * total_q + row / heads] = sum;
 }
 
-// dK, dV: a lane pair is a key, its K and V fragments and both gradients stay in registers; tiles of 64 queries (Q, dO, lse,
-// delta) go through LDS, each read by rows (scores, dP) and by columns (the two gradients).
+// dK, dV of 32 KB keys.  The steps of a workgroup -- tiles of 32 queries of every head of the group -- are dealt to its four
+// waves; a wave streams its tiles (Q, dO, row statistics) through an LDS ring of its own, so there is no barrier in the loop, and
+// reads each by rows (scores, dP) and by columns (the two gradients).  K and V fragments and both gradients of all the keys
+// stay in registers: with KB = 2 every fragment that is read from LDS feeds two products (one for each 32 keys), which halves
+// the LDS traffic that would otherwise bound the loop.  At the end the waves' sums are joined in LDS in wave order.
+template <typename T, int DPAD> struct KeyTile {
+    typedef Tile<T, DPAD, 32> Tl;
+    static constexpr int KB = sizeof(T) * DPAD <= 256 ? 2 : 1, KEYS = 32 * KB;       // registers: 2 KB (fragments + sums) of DPAD columns
+    static constexpr int WAVES = sizeof(T) * DPAD > 256 ? 2 : 4;        // two where four rings would not fit the LDS
+    static constexpr int BUF = 2 * Tl::BYTES + (Stats<T>::N + 1) * 256, PAD = DPAD + 4;
+    static constexpr int RINGS = WAVES * 2 * BUF, JOIN = WAVES * KEYS * PAD * 4, LDS = RINGS > JOIN ? RINGS : JOIN;
+};
+
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DPAD < 128 ? 2 : 1) void attention_dkdv_kernel(Params p)
+__global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
 {
-    typedef Tile<T, DPAD, BN> Tl;
+    typedef KeyTile<T, DPAD> Kt;
+    typedef Tile<T, DPAD, 32> Tl;
     typedef typename Elem<T>::Frag Frag;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    constexpr int STATS = 2 * BN * 4, BUF = 2 * Tl::BYTES + STATS;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // [2 buffers][Q tile, dO tile, lse, delta]
+    constexpr int KB = Kt::KB, KEYS = Kt::KEYS, WAVES = Kt::WAVES;
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [wave][2 buffers][Q tile, dO tile, delta, statistics]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int slots = num_slots(p.nseq, p.total_k, BM);
-    const Work w = work_of(blockIdx.x, slots, p.heads_k, 1);
-    if (w.slot < 0) return;
-    const int s = __builtin_amdgcn_readfirstlane(find_seq(p.cu_k, p.nseq, p.total_k, w.slot, BM, lane));
-    const Seq sq = seq_of(p, s);
-    const int row0 = (w.slot - (sq.k0 / BM + s)) * BM;                    // first key within the sequence
-    if (row0 >= sq.kcap) return;
-    const int kw0 = row0 + wave * 32, ki = kw0 + (lane & 31), shift = sq.lk - sq.lq;
+    const Work w = work_of(blockIdx.x, p.heads_k, 1);
+    const Where where = locate<true>(p, w.number, KEYS, lane);
+    if (!where.ok) return;
+    const Seq sq = where.sq;
+    const int row0 = where.row, shift = sq.lk - sq.lq;                    // first key within the sequence
 
-    Frag kf[DPAD / 16], vf[DPAD / 16];
-    load_row_frags<T, DPAD>(kf, (const T*)p.k + (int64_t)(sq.k0 + ki) * p.k_tok + (int64_t)w.kvh * p.k_head, ki < sq.lk, p.dim, lane);
-    load_row_frags<T, DPAD>(vf, (const T*)p.v + (int64_t)(sq.k0 + ki) * p.v_tok + (int64_t)w.kvh * p.v_head, ki < sq.lk, p.dim, lane);
+    Frag kf[KB][DPAD / 16], vf[KB][DPAD / 16];
+    f32x16 dk[KB][DPAD / 32], dv[KB][DPAD / 32];
+#pragma unroll
+    for (int n = 0; n < KB; ++n) {
+        const int ki = row0 + n * 32 + (lane & 31);
+        load_row_frags<T, DPAD>(kf[n], (const T*)p.k + (int64_t)(sq.k0 + ki) * p.k_tok + (int64_t)w.kvh * p.k_head, ki < sq.lk, p.dim, lane);
+        load_row_frags<T, DPAD>(vf[n], (const T*)p.v + (int64_t)(sq.k0 + ki) * p.v_tok + (int64_t)w.kvh * p.v_head, ki < sq.lk, p.dim, lane);
+#pragma unroll
+        for (int c = 0; c < DPAD / 32; ++c) dk[n][c] = dv[n][c] = f32x16{};
+    }
 
-    // query tiles that see any of the workgroup's keys
-    const int first = p.causal ? max(0, row0 - shift) / BN : 0;
-    const int ntiles = row0 < sq.lk ? max(0, (sq.lq + BN - 1) / BN - first) : 0, steps = ntiles * p.group;
-
-    Filler<T, DPAD, BN, 4> fq, fo;
-    fq.init(p.q_tok, p.dim, wave, lane);
-    fo.init((int64_t)p.heads_q * p.dim, p.dim, wave, lane);
-    auto fill = [&](int it) {
-        const int head = w.kvh * p.group + it / ntiles, r = (first + it % ntiles) * BN, left = sq.lq - r;
+    // query tiles that see any of the keys
+    const int first = p.causal ? max(0, row0 - shift) / 32 : 0;
+    const int ntiles = row0 < sq.lk ? max(0, (sq.lq + 31) / 32 - first) : 0, steps = ntiles * p.group;
+    Filler<T, DPAD, 32, 1> fq, fo;
+    fq.init(p.q_tok, p.dim, 0, lane);
+    fo.init((int64_t)p.heads_q * p.dim, p.dim, 0, lane);
+    char* ring = lds + wave * 2 * Kt::BUF;
+    auto fill = [&](int it, int b) {
+        const int head = w.kvh * p.group + it / ntiles, r = (first + it % ntiles) * 32, left = sq.lq - r;
         const int64_t row = sq.q0 + r;
-        char* buf = lds + (it & 1) * BUF;
+        char* buf = ring + b * Kt::BUF;
         fq.issue((const T*)p.q + row * p.q_tok + (int64_t)head * p.q_head, left, buf);
         fo.issue((const T*)p.go + (row * p.heads_q + head) * p.dim, left, buf + Tl::BYTES);
-        if (wave < 2) {
-            const float* src = (wave ? p.delta : p.lse) + (int64_t)head * p.total_q + row;
-            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), 0, (left < BN ? left : BN) * 4, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LDS_PTR void*)(buf + 2 * Tl::BYTES + wave * BN * 4), 4, lane * 4, 0, 0, 0);
+        // 64 floats each: statistics of rows behind the tile are fetched, too, and not used; those behind the sequence become
+        // 0 (their Q and dO are zeros)
+        const int64_t at = (int64_t)head * p.total_q + row;
+        const int bytes = (left < 64 ? left : 64) * 4;
+#pragma unroll
+        for (int u = 0; u <= Stats<T>::N; ++u) {
+            const float* src = (u == 0 ? p.delta : p.stats + (u - 1) * (int64_t)p.heads_q * p.total_q) + at;
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), 0, bytes, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LDS_PTR void*)(buf + 2 * Tl::BYTES + u * 256), 4, lane * 4, 0, 0, 0);
         }
     };
     const int rbase = Tl::row_base(lane), cbase = Tl::col_base(lane);
-    f32x16 dk[DPAD / 32], dv[DPAD / 32];
+    if (wave < steps) fill(wave, 0);
+    int b = 0;
+    for (int it = wave; it < steps; it += WAVES, b ^= 1) {
+        if (it + WAVES < steps) {
+            wait_lds();
+            fill(it + WAVES, b ^ 1);
+            wait_loads<2 * Tl::LOADS + 1 + Stats<T>::N>();
+        } else {
+            wait_loads<0>();
+        }
+        const int qb = (first + it % ntiles) * 32;
+        const char *qt = ring + b * Kt::BUF, *ot = qt + Tl::BYTES;
+        const float *delta = reinterpret_cast<const float*>(ot + Tl::BYTES), *ref = delta + 64, *inv = ref + 64;
+        f32x16 sc[KB], dp[KB];
 #pragma unroll
-    for (int b = 0; b < DPAD / 32; ++b) dk[b] = dv[b] = f32x16{};
-    if (steps) fill(0);
-    for (int it = 0; it < steps; ++it) {
-        wait_loads<0>();
-        barrier();
-        if (it + 1 < steps) fill(it + 1);
-        const int q0 = (first + it % ntiles) * BN;
-        const char *qt = lds + (it & 1) * BUF, *ot = qt + Tl::BYTES;
-        const float *lse = reinterpret_cast<const float*>(ot + Tl::BYTES), *delta = lse + BN;
+        for (int n = 0; n < KB; ++n) sc[n] = dp[n] = f32x16{};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int qb = q0 + b * 32;
-            if (kw0 >= sq.lk || (p.causal && kw0 > qb + 31 + shift)) continue;       // nothing to see for this wave
-            f32x16 sc = f32x16{}, dp = f32x16{};
+        for (int d = 0; d < DPAD / 16; ++d) {
+            const Frag f = Tl::row(qt, rbase, 0, d);
 #pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) sc = Elem<T>::mma(Tl::row(qt, rbase, b, d), kf[d], sc);
+            for (int n = 0; n < KB; ++n) sc[n] = Elem<T>::mma(f, kf[n][d], sc[n]);
+        }
 #pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) dp = Elem<T>::mma(Tl::row(ot, rbase, b, d), vf[d], dp);
-            const bool edge = p.causal && kw0 + 31 > qb + shift;
+        for (int d = 0; d < DPAD / 16; ++d) {
+            const Frag f = Tl::row(ot, rbase, 0, d);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f4 ls = *reinterpret_cast<const f4*>(lse + b * 32 + r * 8 + half * 4);
-                const f4 de = *reinterpret_cast<const f4*>(delta + b * 32 + r * 8 + half * 4);
+            for (int n = 0; n < KB; ++n) dp[n] = Elem<T>::mma(f, vf[n][d], dp[n]);
+        }
+        const bool edge = p.causal && row0 + KEYS - 1 > qb + shift;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const f4 rf = *reinterpret_cast<const f4*>(ref + r * 8 + half * 4), de = *reinterpret_cast<const f4*>(delta + r * 8 + half * 4);
+            f4 iv;
+            if constexpr (Stats<T>::N == 2) iv = *reinterpret_cast<const f4*>(inv + r * 8 + half * 4);
+#pragma unroll
+            for (int n = 0; n < KB; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float pr = __builtin_amdgcn_exp2f(fmaf(sc[r * 4 + i], p.scale_log2, -ls[i]));
-                    const float ds = pr * (dp[r * 4 + i] - de[i]);
-                    const bool hidden = edge && ki > qb + r * 8 + half * 4 + i + shift;
-                    sc[r * 4 + i] = hidden ? 0.f : pr;
-                    dp[r * 4 + i] = hidden ? 0.f : ds;
+                    float pr = score_exp<T>(sc[n][r * 4 + i], p.scale_log2, rf[i]);
+                    if constexpr (Stats<T>::N == 2) pr *= iv[i];
+                    sc[n][r * 4 + i] = pr;
+                    dp[n][r * 4 + i] = pr * (dp[n][r * 4 + i] - de[i]);
                 }
-            }
+        }
+        if (edge) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag pf = frag_of<T>(sc, k), df = frag_of<T>(dp, k);
+            for (int n = 0; n < KB; ++n)
 #pragma unroll
-                for (int c = 0; c < DPAD / 32; ++c) {
-                    dv[c] = Elem<T>::mma(Tl::col(ot, cbase, c, b * 2 + k), pf, dv[c]);
-                    dk[c] = Elem<T>::mma(Tl::col(qt, cbase, c, b * 2 + k), df, dk[c]);
+                for (int i = 0; i < 16; ++i)
+                    if (row0 + n * 32 + (lane & 31) > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[n][i] = dp[n][i] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            Frag pf[KB], df[KB];
+#pragma unroll
+            for (int n = 0; n < KB; ++n) { pf[n] = frag_of<T>(sc[n], k); df[n] = frag_of<T>(dp[n], k); }
+#pragma unroll
+            for (int c = 0; c < DPAD / 32; ++c) {
+                const Frag fo_ = Tl::col(ot, cbase, c, k), fq_ = Tl::col(qt, cbase, c, k);
+#pragma unroll
+                for (int n = 0; n < KB; ++n) {
+                    dv[n][c] = Elem<T>::mma(fo_, pf[n], dv[n][c]);
+                    dk[n][c] = Elem<T>::mma(fq_, df[n], dk[n][c]);
                 }
             }
         }
     }
-    if (ki >= sq.kcap) return;
-    const bool live = ki < sq.lk;                     // rows of the slot behind its keys get zeros
-    const int64_t at = ((int64_t)(sq.k0 + ki) * p.heads_k + w.kvh) * p.dim;
+
+    // join: [wave][key][dim] fp32 in LDS, dV first, then dK
+    float* joined = reinterpret_cast<float*>(lds);
 #pragma unroll
-    for (int c = 0; c < DPAD / 32; ++c)
+    for (int which = 0; which < 2; ++which) {
+        barrier();                                    // the rings are done with, or the sums of dV have been read
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = c * 32 + r * 8 + half * 4;
-            if (d >= p.dim) continue;
-            float a[4], b[4];
+        for (int n = 0; n < KB; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i] = live ? dk[c][r * 4 + i] * p.scale : 0.f; b[i] = live ? dv[c][r * 4 + i] : 0.f; }
-            store4((T*)p.dk + at + d, a[0], a[1], a[2], a[3]);
-            store4((T*)p.dv + at + d, b[0], b[1], b[2], b[3]);
+            for (int c = 0; c < DPAD / 32; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x16& a = which ? dk[n][c] : dv[n][c];
+                    *reinterpret_cast<f4*>(joined + (wave * KEYS + n * 32 + (lane & 31)) * Kt::PAD + c * 32 + r * 8 + half * 4) =
+                        f4{a[r * 4], a[r * 4 + 1], a[r * 4 + 2], a[r * 4 + 3]};
+                }
+        __syncthreads();
+        const float f = which ? p.scale : 1.f;
+        for (int e = threadIdx.x; e < KEYS * (DPAD / 4); e += 64 * WAVES) {
+            const int key = e / (DPAD / 4), d = e % (DPAD / 4) * 4, ki = row0 + key;
+            if (ki >= sq.kcap || d >= p.dim) continue;
+            f4 v = {0.f, 0.f, 0.f, 0.f};
+            if (ki < sq.lk)                           // rows of the slot behind its keys get zeros
+#pragma unroll
+                for (int u = 0; u < WAVES; ++u) v += *reinterpret_cast<const f4*>(joined + (u * KEYS + key) * Kt::PAD + d);
+            store4((T*)(which ? p.dk : p.dv) + ((int64_t)(sq.k0 + ki) * p.heads_k + w.kvh) * p.dim + d, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
         }
+    }
 }
 
-// dQ: as the forward, with dO beside Q in registers and K read by columns, too
+// dQ: as the forward, with dO beside Q in registers and K read by columns, too.
 template <typename T, int DPAD>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(Params p)
 {
@@ -145,13 +209,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     typedef typename Elem<T>::Frag Frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];            // [2 buffers][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int slots = num_slots(p.nseq, p.total_q, BM);
-    const Work w = work_of(blockIdx.x, slots, p.heads_k, p.group);
-    if (w.slot < 0) return;
-    const int s = __builtin_amdgcn_readfirstlane(find_seq(p.cu_q, p.nseq, p.total_q, w.slot, BM, lane));
-    const Seq sq = seq_of(p, s);
-    const int row0 = (w.slot - (sq.q0 / BM + s)) * BM;
-    if (row0 >= sq.lq) return;
+    const Work w = work_of(blockIdx.x, p.heads_k, p.group);
+    const Where at = locate<false>(p, w.number, BM, lane);
+    if (!at.ok) return;
+    const Seq sq = at.sq;
+    const int row0 = at.row;
     const int head = w.kvh * p.group + w.g, shift = sq.lk - sq.lq;
     const int qi = row0 + wave * 32 + (lane & 31);
     const bool present = qi < sq.lq;
@@ -160,8 +222,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     Frag qf[DPAD / 16], of[DPAD / 16];
     load_row_frags<T, DPAD>(qf, (const T*)p.q + (int64_t)(sq.q0 + qi) * p.q_tok + (int64_t)head * p.q_head, present, p.dim, lane);
     load_row_frags<T, DPAD>(of, (const T*)p.go + orow, present, p.dim, lane);
-    const float lse = present ? p.lse[(int64_t)head * p.total_q + sq.q0 + qi] : INFINITY;
-    const float delta = present ? p.delta[(int64_t)head * p.total_q + sq.q0 + qi] : 0.f;
+    const int64_t stat = (int64_t)head * p.total_q + sq.q0 + qi;
+    const float ref = present ? p.stats[stat] : INFINITY, delta = present ? p.delta[stat] : 0.f;
 
     const int see = p.causal ? min(sq.lk, qi + 1 + shift) : sq.lk;
     const int see_first = p.causal ? min(sq.lk, row0 + wave * 32 + 1 + shift) : sq.lk;
@@ -201,26 +263,38 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
             for (int d = 0; d < DPAD / 16; ++d) dp = Elem<T>::mma(Tl::row(vt, rbase, b, d), of[d], dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float pr = __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale_log2, -lse));
-                const float ds = pr * (dp[i] - delta);
-                dp[i] = edge && key0 + b * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see ? 0.f : ds;
+                const bool hidden = edge && key0 + b * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see;
+                dp[i] = hidden ? 0.f : score_exp<T>(sc[i], p.scale_log2, ref) * (dp[i] - delta);
             }
+            if constexpr (sizeof(T) == 4) {
+                // 32 keys are summed by themselves first, see the forward
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag df = frag_of<T>(dp, k);
+                for (int c = 0; c < DPAD / 32; ++c) {
+                    f32x16 part = f32x16{};
 #pragma unroll
-                for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(kt, cbase, c, b * 2 + k), df, acc[c]);
+                    for (int k = 0; k < 2; ++k) part = Elem<T>::mma(Tl::col(kt, cbase, c, b * 2 + k), frag_of<T>(dp, k), part);
+                    acc[c] += part;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const Frag df = frag_of<T>(dp, k);
+#pragma unroll
+                    for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(kt, cbase, c, b * 2 + k), df, acc[c]);
+                }
             }
         }
     }
     if (!present) return;
+    float f = p.scale;
+    if (sizeof(T) == 4) f *= p.stats[(int64_t)p.heads_q * p.total_q + stat];
     T* out = (T*)p.dq + orow;
 #pragma unroll
     for (int c = 0; c < DPAD / 32; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int d = c * 32 + r * 8 + half * 4;
-            if (d < p.dim) store4(out + d, acc[c][r * 4] * p.scale, acc[c][r * 4 + 1] * p.scale, acc[c][r * 4 + 2] * p.scale, acc[c][r * 4 + 3] * p.scale);
+            if (d < p.dim) store4(out + d, acc[c][r * 4] * f, acc[c][r * 4 + 1] * f, acc[c][r * 4 + 2] * f, acc[c][r * 4 + 3] * f);
         }
 }
 
@@ -233,13 +307,14 @@ SEMPYR_BWD_KERNELS(bf16, 32) SEMPYR_BWD_KERNELS(bf16, 64) SEMPYR_BWD_KERNELS(bf1
 
 template <typename T, int DPAD>
 static int launch_bwd_d(const Params& p, hipStream_t st) {
-    const int64_t bk = work_blocks(num_slots(p.nseq, p.total_k, BM), p.heads_k, 1);
-    const int64_t bq = work_blocks(num_slots(p.nseq, p.total_q, BM), p.heads_k, p.group);
+    typedef KeyTile<T, DPAD> Kt;
+    const int64_t bk = work_blocks(num_tiles(p.nseq, p.total_k, Kt::KEYS), p.heads_k, 1);
+    const int64_t bq = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
     if (bk > 0x7FFFFFFF || bq > 0x7FFFFFFF) SEMPYR_FAIL("attention_bwd: too many tiles");
-    const int tile = Tile<T, DPAD, BN>::BYTES, lds_kv = 4 * tile + 4 * BN * 4, lds_q = 4 * tile;
+    const int lds_q = 4 * Tile<T, DPAD, BN>::BYTES;
     if (p.total_k > 0) {
-        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, lds_kv)) return rc;
-        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 256, lds_kv, st>>>(p);
+        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, Kt::LDS)) return rc;
+        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 64 * Kt::WAVES, Kt::LDS, st>>>(p);
         SEMPYR_CHECK_LAUNCH();
     }
     if (p.total_q > 0) {
@@ -255,7 +330,7 @@ static int launch_bwd_t(const Params& p, float* delta, hipStream_t st) {
     const int64_t rows = (int64_t)p.total_q * p.heads_q;
     if (rows > 0) {
         if (rows > 0x7FFFFFFFll * 16) SEMPYR_FAIL("attention_bwd: too many rows");
-        attention_delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>((const T*)p.go, (const T*)p.o, delta, rows, p.total_q, p.heads_q, p.dim);
+        attention_delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>((const T*)p.go, (const T*)p.o, (const T*)p.o_low, delta, rows, p.total_q, p.heads_q, p.dim);
         SEMPYR_CHECK_LAUNCH();
     }
     if (p.dim <= 32) return launch_bwd_d<T, 32>(p, st);

@@ -18,13 +18,11 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
     typedef typename Elem<T>::Frag Frag;
     extern __shared__ __attribute__((aligned(16))) char lds[];            // [2 buffers][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int slots = num_slots(p.nseq, p.total_q, BM);
-    const Work w = work_of(blockIdx.x, slots, p.heads_k, p.group);
-    if (w.slot < 0) return;
-    const int s = __builtin_amdgcn_readfirstlane(find_seq(p.cu_q, p.nseq, p.total_q, w.slot, BM, lane));
-    const Seq sq = seq_of(p, s);
-    const int row0 = (w.slot - (sq.q0 / BM + s)) * BM;                    // within the sequence
-    if (row0 >= sq.lq) return;
+    const Work w = work_of(blockIdx.x, p.heads_k, p.group);
+    const Where at = locate<false>(p, w.number, BM, lane);
+    if (!at.ok) return;
+    const Seq sq = at.sq;
+    const int row0 = at.row;                                          // within the sequence
     const int head = w.kvh * p.group + w.g, shift = sq.lk - sq.lq;
     const int qi = row0 + wave * 32 + (lane & 31);
     const bool present = qi < sq.lq;
@@ -81,47 +79,58 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float base = mx == -INFINITY ? 0.f : mx * p.scale_log2;       // a row that has seen no key yet
-        const float alpha = __builtin_amdgcn_exp2f(m * p.scale_log2 - base);
+        const float base = score_ref<T>(mx, p.scale_log2);                  // 0 for a row that has seen no key yet
+        const float alpha = score_exp<T>(m, p.scale_log2, base);
         m = mx;
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                sc[b][i] = __builtin_amdgcn_exp2f(fmaf(sc[b][i], p.scale_log2, -base));
+                sc[b][i] = score_exp<T>(sc[b][i], p.scale_log2, base);
                 sum += sc[b][i];
             }
         l = l * alpha + sum;
+        if constexpr (sizeof(T) == 4) {
+            // a tile's products are summed by themselves first: a chain over all keys would lose bits with its length
 #pragma unroll
-        for (int b = 0; b < DPAD / 32; ++b)
+            for (int b = 0; b < DPAD / 32; ++b) {
+                f32x16 part = f32x16{};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
+                for (int k = 0; k < 4; ++k) part = Elem<T>::mma(Tl::col(vt, cbase, b, k), frag_of<T>(sc[k / 2], k % 2), part);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const Frag pf = frag_of<T>(sc[k / 2], k % 2);
+                for (int i = 0; i < 16; ++i) acc[b][i] = fmaf(acc[b][i], alpha, part[i]);
+            }
+        } else {
 #pragma unroll
-            for (int b = 0; b < DPAD / 32; ++b) acc[b] = Elem<T>::mma(Tl::col(vt, cbase, b, k), pf, acc[b]);
+            for (int b = 0; b < DPAD / 32; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const Frag pf = frag_of<T>(sc[k / 2], k % 2);
+#pragma unroll
+                for (int b = 0; b < DPAD / 32; ++b) acc[b] = Elem<T>::mma(Tl::col(vt, cbase, b, k), pf, acc[b]);
+            }
         }
     }
     l += __shfl_xor(l, 32, 64);                      // each lane half has summed its own keys
     if (!present) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;      // no key: zeros
-    T* out = (T*)p.o + ((int64_t)(sq.q0 + qi) * p.heads_q + head) * p.dim;
+    const int64_t out = ((int64_t)(sq.q0 + qi) * p.heads_q + head) * p.dim;
 #pragma unroll
     for (int b = 0; b < DPAD / 32; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int d = b * 32 + r * 8 + half * 4;
-            if (d < p.dim) store4(out + d, acc[b][r * 4] * inv, acc[b][r * 4 + 1] * inv, acc[b][r * 4 + 2] * inv, acc[b][r * 4 + 3] * inv);
+            if (d < p.dim) store_out<T>(p, out + d, acc[b][r * 4] * inv, acc[b][r * 4 + 1] * inv, acc[b][r * 4 + 2] * inv, acc[b][r * 4 + 3] * inv);
         }
-    // a row without keys gets +infinity: its probabilities are recomputed as exp2(x - infinity) = 0
-    if (p.lse && half == 0) p.lse[(int64_t)head * p.total_q + sq.q0 + qi] = l == 0.f ? INFINITY : m * p.scale_log2 + __log2f(l);
+    if (p.stats && half == 0) Stats<T>::store(p, (int64_t)head * p.total_q + sq.q0 + qi, m, l);
 }
 
 template <typename T, int DPAD>
 static int launch_fwd_d(const Params& p, hipStream_t st) {
-    const int64_t blocks = work_blocks(num_slots(p.nseq, p.total_q, BM), p.heads_k, p.group);
+    const int64_t blocks = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
     if (blocks > 0x7FFFFFFF) SEMPYR_FAIL("attention_fwd: too many tiles");
     const int bytes = 4 * Tile<T, DPAD, BN>::BYTES;
     if (int rc = allow_lds((const void*)attention_fwd_kernel<T, DPAD>, bytes)) return rc;

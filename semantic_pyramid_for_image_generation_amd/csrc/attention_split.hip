@@ -13,17 +13,19 @@ namespace attn {
 
 constexpr int BK = 32;
 
-// Four waves, two where four rings would not fit the 160 KiB of a CU.
+// Two waves a workgroup: 64 KiB of rings for 16-bit heads of 128, so a second workgroup's start and end (search, first tiles,
+// join) overlap this one's stream.  Eight requests' tokens against up to 32768 keys, 32/8 heads of 128, bf16 (549 MB): 2 waves
+// and 1024 workgroups 120 us (4.6 TB/s), 4 and 512 119, 2 and 2048 127, 4 and 2048 175.
 template <typename T, int DPAD> struct Split {
     typedef Tile<T, DPAD, BK> Tl;
-    static constexpr int WAVES = sizeof(T) * DPAD > 256 ? 2 : 4;
+    static constexpr int WAVES = 2;
     static constexpr int RING = 4 * Tl::BYTES, PAD = DPAD + 4;       // ring: two buffers of a K and a V tile
     static constexpr int STATS = WAVES * 32 * 2 * 4, LDS = WAVES * RING + STATS;
     static_assert(WAVES * 32 * PAD * 4 <= WAVES * RING, "the joined results reuse the rings");
 };
 
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p, SplitPlan plan, float* __restrict__ part_o,
+__global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, SplitPlan plan, float* __restrict__ part_o,
                                                                   float* __restrict__ part_ml)
 {
     typedef Split<T, DPAD> Sp;
@@ -36,12 +38,12 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p, Split
     int idx = blockIdx.x;
     const int chunk = idx % plan.head_chunks; idx /= plan.head_chunks;
     const int kvh = idx % p.heads_k; idx /= p.heads_k;
-    const int split = idx % plan.splits, slot = idx / plan.splits;
+    const int split = idx % plan.splits, number = idx / plan.splits;
     const int QT = plan.queries;                     // queries of a tile
-    const int s = __builtin_amdgcn_readfirstlane(find_seq(p.cu_q, p.nseq, p.total_q, slot, QT, lane));
-    const Seq sq = seq_of(p, s);
-    const int row0 = (slot - (sq.q0 / QT + s)) * QT;
-    if (row0 >= sq.lq) return;
+    const Where at = locate<false>(p, number, QT, lane);
+    if (!at.ok) return;
+    const Seq sq = at.sq;
+    const int row0 = at.row;
     const int shift = sq.lk - sq.lq, col = lane & 31;
     // column -> query and head
     auto query_of = [&](int c) { return row0 + c / plan.heads; };
@@ -102,13 +104,13 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p, Split
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[i]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float base = mx == -INFINITY ? 0.f : mx * p.scale_log2;
-        const float alpha = __builtin_amdgcn_exp2f(m * p.scale_log2 - base);
+        const float base = score_ref<T>(mx, p.scale_log2);
+        const float alpha = score_exp<T>(m, p.scale_log2, base);
         m = mx;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale_log2, -base));
+            sc[i] = score_exp<T>(sc[i], p.scale_log2, base);
             sum += sc[i];
         }
         l = l * alpha + sum;
@@ -162,51 +164,60 @@ __global__ __launch_bounds__(256, 1) void attention_split_kernel(Params p, Split
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += f[w] * *reinterpret_cast<const f4*>(joined + (w * 32 + c) * Sp::PAD + d);
         v *= inv;
-        if (whole) store4((T*)p.o + row * p.dim + d, v[0], v[1], v[2], v[3]);
+        if (whole) store_out<T>(p, row * p.dim + d, v[0], v[1], v[2], v[3]);
         else if (total != 0.f) *reinterpret_cast<f4*>(part_o + (split * rows + row) * p.dim + d) = v;
     }
     if (threadIdx.x % PER_COL == 0) {
         if (!whole) {
             part_ml[(split * rows + row) * 2] = top;
             part_ml[(split * rows + row) * 2 + 1] = total;
-        } else if (p.lse) {
-            p.lse[(int64_t)head * p.total_q + token] = total == 0.f ? INFINITY : top * p.scale_log2 + __log2f(total);
+        } else if (p.stats) {
+            Stats<T>::store(p, (int64_t)head * p.total_q + token, top, total);
         }
     }
 }
 
-// Joins the workgroups' partial results: 32 lanes a row.
+// Joins the partial results of `splits` workgroups: a workgroup a row, 32 lanes hold the row's elements, the eight groups of 32
+// lanes take every eighth split (the loads of a thread are independent), a sum over the groups in order ends it.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join_kernel(Params p, int splits, const float* __restrict__ part_o,
                                                              const float* __restrict__ part_ml)
 {
     typedef float f4 __attribute__((ext_vector_type(4)));
-    const int64_t rows = (int64_t)p.total_q * p.heads_q, row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-    if (row >= rows) return;
-    const int lane = threadIdx.x % 32;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    __shared__ f4 sums[8][32];
+    __shared__ float totals[8];
+    const int64_t rows = (int64_t)p.total_q * p.heads_q, row = blockIdx.x;
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32, d = lane * 4;
+    const f2* ml = reinterpret_cast<const f2*>(part_ml);
     float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_ml[(s * rows + row) * 2]);
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, ml[s * rows + row][0]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     float total = 0.f;
     f4 v = {0.f, 0.f, 0.f, 0.f};
-    const int d = lane * 4;
-    for (int s = 0; s < splits; ++s) {
-        const float m = part_ml[(s * rows + row) * 2], l = part_ml[(s * rows + row) * 2 + 1];
-        if (l == 0.f) continue;                      // no key in this split; its partial sums were not written
-        const float f = __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
-        total += f * l;
+#pragma unroll 4
+    for (int s = group; s < splits; s += 8) {
+        const f2 x = ml[s * rows + row];
+        if (x[1] == 0.f) continue;                   // no key in this split; its partial sums were not written
+        const float f = __builtin_amdgcn_exp2f((x[0] - top) * p.scale_log2);
+        total += f * x[1];
         if (d < p.dim) v += f * *reinterpret_cast<const f4*>(part_o + (s * rows + row) * p.dim + d);
     }
+    sums[group][lane] = v;
+    if (lane == 0) totals[group] = total;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < 8; ++g) { v += sums[g][lane]; total += totals[g]; }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (d < p.dim) store4((T*)p.o + row * p.dim + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-    if (p.lse && lane == 0)
-        p.lse[(row % p.heads_q) * p.total_q + row / p.heads_q] = total == 0.f ? INFINITY : top * p.scale_log2 + __log2f(total);
+    if (d < p.dim) store_out<T>(p, row * p.dim + d, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    if (p.stats && lane == 0) Stats<T>::store(p, (row % p.heads_q) * p.total_q + row / p.heads_q, top, total);
 }
 
 // A tile of the one-pass kernel holds 128 queries of one head; where those tiles cannot occupy the 256 CUs, the rows are
 // packed and the keys split instead.
-SplitPlan plan_split(int dtype, const Params& p) {
+SplitPlan plan_split(const Params& p) {
     SplitPlan s = {};
     const int64_t tiles = ((int64_t)p.total_q / 128 + p.nseq) * p.heads_q;
     s.head_chunks = (p.group + 31) / 32;
@@ -215,9 +226,8 @@ SplitPlan plan_split(int dtype, const Params& p) {
     const bool few_queries = (int64_t)p.total_q <= (int64_t)s.queries * p.nseq;        // a tile a sequence holds them on average
     if (p.total_q == 0 || (tiles > 256 && !few_queries)) return s;
     const int64_t packed = ((int64_t)(p.total_q + s.queries - 1) / s.queries + (p.nseq > 1 ? p.nseq : 0) / 2) * p.heads_k * s.head_chunks;
-    const int waves = dtype == SEMPYR_F32 && p.dim > 64 ? 2 : 4;
-    const int64_t keys = p.nseq > 0 ? p.total_k / p.nseq : 0, most = (keys + BK * waves - 1) / (BK * waves);      // a tile a wave
-    int64_t n = (2048 + packed - 1) / packed;
+    const int64_t keys = p.nseq > 0 ? p.total_k / p.nseq : 0, most = (keys + 2 * BK - 1) / (2 * BK);      // a tile a wave
+    int64_t n = (1024 + packed - 1) / packed;
     n = n < most ? n : most;
     s.splits = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
     return s;
@@ -227,14 +237,14 @@ template <typename T, int DPAD>
 static int launch_split_d(const Params& p, const SplitPlan& plan, float* ws, hipStream_t st) {
     typedef Split<T, DPAD> Sp;
     const int64_t rows = (int64_t)p.total_q * p.heads_q;
-    const int64_t blocks = (int64_t)num_slots(p.nseq, p.total_q, plan.queries) * plan.splits * p.heads_k * plan.head_chunks;
-    if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFFll * 8) SEMPYR_FAIL("attention_fwd: too many tiles");
+    const int64_t blocks = (int64_t)num_tiles(p.nseq, p.total_q, plan.queries) * plan.splits * p.heads_k * plan.head_chunks;
+    if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFF) SEMPYR_FAIL("attention_fwd: too many tiles");
     float* ml = ws ? ws + plan.splits * rows * p.dim : nullptr;
     if (int rc = allow_lds((const void*)attention_split_kernel<T, DPAD>, Sp::LDS)) return rc;
     attention_split_kernel<T, DPAD><<<(unsigned)blocks, 64 * Sp::WAVES, Sp::LDS, st>>>(p, plan, ws, ml);
     SEMPYR_CHECK_LAUNCH();
     if (plan.splits > 1) {
-        attention_join_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, plan.splits, ws, ml);
+        attention_join_kernel<T><<<(unsigned)rows, 256, 0, st>>>(p, plan.splits, ws, ml);
         SEMPYR_CHECK_LAUNCH();
     }
     return 0;

@@ -27,7 +27,8 @@ struct Params {
     const void *q, *k, *v;                                   // [rows][heads][dim], strides in elements
     int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
     void* o;                                                 // contiguous [total_q][heads_q][dim]
-    float* lse;                                              // [heads_q][total_q]: log2 of a row's sum of exponentials, or null
+    void* o_low;                                             // 16-bit types: what rounding took from o, for delta; or null
+    float* stats;                                            // rows' softmax statistics for the backward pass (see Stats), or null
     const void* go;                                          // backward: gradient of o, contiguous
     const float* delta;                                      // backward: [heads_q][total_q] rowsum(go * o)
     void *dq, *dk, *dv;                                      // backward: contiguous
@@ -188,6 +189,35 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
     *reinterpret_cast<V*>(p) = V{(T)a, (T)b, (T)c, (T)d};
 }
 
+// What the forward leaves of a row's softmax.  16-bit types: lse = c m + log2(sum), from which P = exp2(c s - lse); its rounding
+// (2^-24 of about 10) is far below theirs.  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
+// exp2(c (s - m)) / sum: with lse the gradients of 1024 keys were off by 9e-7, twice what the products themselves leave.
+template <typename T> struct Stats {
+    static constexpr int N = sizeof(T) == 4 ? 2 : 1;
+    static __device__ __forceinline__ void store(const Params& p, int64_t at, float m, float sum) {
+        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum);      // no key: P = exp2(-infinity)
+        else {
+            p.stats[at] = sum == 0.f ? INFINITY : m;
+            p.stats[(int64_t)p.heads_q * p.total_q + at] = sum == 0.f ? 0.f : 1.f / sum;
+        }
+    }
+};
+// exponential of a score against a row's reference x (forward: c m for 16-bit types, m for fp32).  fp32 subtracts first: exact
+// next to the maximum, so that a row with one key is that key's value to the bit.
+template <typename T>
+__device__ __forceinline__ float score_exp(float s, float c, float x) {
+    return sizeof(T) == 4 ? __builtin_amdgcn_exp2f((s - x) * c) : __builtin_amdgcn_exp2f(fmaf(s, c, -x));
+}
+template <typename T>
+__device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c; }
+
+// 4 consecutive elements of the output and, where it is asked for, of what their rounding left
+template <typename T>
+__device__ __forceinline__ void store_out(const Params& p, int64_t at, float a, float b, float c, float d) {
+    store4((T*)p.o + at, a, b, c, d);
+    if (sizeof(T) == 2 && p.o_low) store4((T*)p.o_low + at, a - (float)(T)a, b - (float)(T)b, c - (float)(T)c, d - (float)(T)d);
+}
+
 // ---------------------------------------------------------------------------------------------- packed sequences
 // Sequence s covers rows cu[s] .. cu[s + 1] - 1; the first entry counts as 0, rows behind the last entry form one more,
 // key-less sequence (their results are zeros).  Every entry is clamped to the tensor, so a bad table reads nothing outside.
@@ -214,37 +244,106 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int s) {
     return q;
 }
 
-// Tiles of R rows are numbered so that sequence s owns slots cu[s] / R + s .. (at least as many as it has tiles; the rest are
-// empty): no table has to be built and lengths may change between replays of a captured graph.  The search probes 64
-// entries at a time.
-__device__ __forceinline__ int find_seq(const int32_t* cu, int nseq, int total, int slot, int R, int lane) {
-    int lo = 0, hi = nseq;
-    while (lo < hi) {
-        const int step = (hi - lo + 63) / 64, c = lo + (lane + 1) * step;
-        const bool ok = c <= hi && row_bound(cu, c, nseq, total) / R + c <= slot;
-        lo += __popcll(__ballot(ok)) * step;
-        hi = lo + step - 1 < hi ? lo + step - 1 : hi;
-    }
-    return lo;
+// inclusive prefix sum over the wave (data-parallel primitives: no LDS)
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // last lane of row 0 / 2 into row 1 / 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // lane 31 into rows 2 and 3
+    return v;
 }
-__host__ __device__ inline int num_slots(int nseq, int total, int R) { return total / R + nseq + 1; }
 
-// Workgroup -> (slot, kv head, head in group).  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD gets
-// whole kv heads where there are enough, else every X-th slot of one, so that K and V of a head are read into few L2s; within
-// an XCD the heads of a group come next to each other, and late slots (the long rows of a causal mask) come first.
-struct Work { int slot, kvh, g; };
-__host__ __device__ inline int xcd_classes(int heads_k) { return heads_k % 8 == 0 ? 8 : heads_k % 4 == 0 ? 4 : heads_k % 2 == 0 ? 2 : 1; }
-static inline int64_t work_blocks(int slots, int heads_k, int inner) {
-    const int g = xcd_classes(heads_k), x = 8 / g;
-    return 8ll * ((slots + x - 1) / x) * (heads_k / g) * inner;
+// Tile number -> sequence and first row of the tile, for tiles of R rows of the queries (BY_KEYS: of the key slots).
+// No table has to be built and lengths may change between replays of a captured graph.
+//  * Up to 63 sequences (a lane each, rows behind the last one are one more): tiles are numbered exactly and by falling load
+//    -- the keys a query tile sees, the queries that see a key tile -- so that the longest go first.  A tile's load is found by
+//    bisection over 32 levels of the loads, each probe counts the tiles of all sequences at or above a level.
+//  * More: sequence s owns the numbers cu[s] / R + s .., at least as many as it has tiles (the rest are empty), the numbers
+//    run backwards; the search probes 64 entries at a time.
+struct Where { int s, row; bool ok; Seq sq; };
+
+template <bool BY_KEYS>
+__device__ __forceinline__ Where locate(const Params& p, int number, int R, int lane) {
+    Where w;
+    const int total = BY_KEYS ? p.total_k : p.total_q;
+    const int32_t* cu = BY_KEYS ? p.cu_k : p.cu_q;
+    if (p.nseq > 63) {
+        const int slot = total / R + p.nseq - number;
+        int lo = 0, hi = p.nseq;
+        while (lo < hi) {
+            const int step = (hi - lo + 63) / 64, c = lo + (lane + 1) * step;
+            const bool ok = c <= hi && row_bound(cu, c, p.nseq, total) / R + c <= slot;
+            lo += __popcll(__ballot(ok)) * step;
+            hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+        }
+        w.s = __builtin_amdgcn_readfirstlane(lo);
+        w.sq = seq_of(p, w.s);
+        w.row = (slot - ((BY_KEYS ? w.sq.k0 : w.sq.q0) / R + w.s)) * R;
+        w.ok = slot >= 0 && w.row >= 0 && w.row < (BY_KEYS ? w.sq.kcap : w.sq.lq);
+        return w;
+    }
+    Seq sq = {0, 0, 0, 0, 0};
+    if (lane <= p.nseq) sq = seq_of(p, lane);
+    const int rows = BY_KEYS ? sq.kcap : sq.lq, n = (rows + R - 1) / R, shift = sq.lk - sq.lq;
+    // tiles of this lane's sequence whose load is at least x; the loads fall with the tile's rank
+    auto count = [&](int x) {
+        if (x <= 0) return n;
+        int c;
+        if (BY_KEYS) c = x > sq.lq ? 0 : !p.causal ? (sq.lk + R - 1) / R : (min(sq.lk - 1, sq.lq - x + shift) + R) / R;
+        else c = !p.causal ? (sq.lk >= x ? n : 0) : n - (max(0, x - shift) + R - 1) / R;
+        return max(0, min(n, c));
+    };
+    const int all = __builtin_amdgcn_readlane(wave_scan(n), 63);
+    w.ok = number < all;
+    if (!w.ok) return w;
+    int top = lane <= p.nseq ? (BY_KEYS ? sq.lq : sq.lk) : 0;            // no load is larger
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+    const int level = max(R, top / 32 + 1);
+    int lo = 0, hi = 33;                                                 // count(lo level) > number >= count(hi level)
+    if (p.nseq == 1 && !BY_KEYS && number < __builtin_amdgcn_readlane(n, 0)) {      // one sequence: late tiles first
+        w.s = 0;
+        w.row = (__builtin_amdgcn_readlane(n, 0) - 1 - number) * R;
+    } else {
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (__builtin_amdgcn_readlane(wave_scan(count(mid * level)), 63) > number) lo = mid; else hi = mid;
+        }
+        const int above = count((lo + 1) * level), sum_above = __builtin_amdgcn_readlane(wave_scan(above), 63);
+        const int mine = count(lo * level) - above, upto = wave_scan(mine), r = number - sum_above;
+        const unsigned long long after = __ballot(upto > r);             // first lane that reaches past r
+        w.s = __builtin_amdgcn_readfirstlane(__ffsll(after) - 1);
+        const int rank = above + r - (upto - mine);                      // in its sequence, by falling load
+        w.row = __builtin_amdgcn_readlane(!BY_KEYS && p.causal ? n - 1 - rank : rank, w.s) * R;
+    }
+    w.sq.q0 = __builtin_amdgcn_readlane(sq.q0, w.s);
+    w.sq.lq = __builtin_amdgcn_readlane(sq.lq, w.s);
+    w.sq.k0 = __builtin_amdgcn_readlane(sq.k0, w.s);
+    w.sq.lk = __builtin_amdgcn_readlane(sq.lk, w.s);
+    w.sq.kcap = __builtin_amdgcn_readlane(sq.kcap, w.s);
+    return w;
 }
-__device__ __forceinline__ Work work_of(int block, int slots, int heads_k, int inner) {
+// numbers that have to be launched: the exact count is only known on the device
+__host__ __device__ inline int num_tiles(int nseq, int total, int R) { return total / R + nseq + 1; }
+
+// Workgroup -> (tile number, kv head, head in group).  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD
+// gets whole kv heads where there are enough, else every X-th tile of one, so that K and V of a head are read into few L2s;
+// within an XCD the heads of a group come next to each other.
+struct Work { int number, kvh, g; };
+__host__ __device__ inline int xcd_classes(int heads_k) { return heads_k % 8 == 0 ? 8 : heads_k % 4 == 0 ? 4 : heads_k % 2 == 0 ? 2 : 1; }
+static inline int64_t work_blocks(int tiles, int heads_k, int inner) {
+    const int g = xcd_classes(heads_k), x = 8 / g;
+    return 8ll * ((tiles + x - 1) / x) * (heads_k / g) * inner;
+}
+__device__ __forceinline__ Work work_of(int block, int heads_k, int inner) {
     const int cls = xcd_classes(heads_k), x = 8 / cls, per = heads_k / cls;
     const int xcd = block & 7, j = block >> 3;
     Work w;
     w.g = j % inner;
     w.kvh = xcd % cls + cls * (j / inner % per);
-    w.slot = slots - 1 - (j / inner / per * x + xcd / cls);
+    w.number = j / inner / per * x + xcd / cls;
     return w;
 }
 

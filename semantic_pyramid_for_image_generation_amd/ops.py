@@ -2021,30 +2021,33 @@ class _Attention(Function):
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
             len_k = len_k if len_k is None else len_k.contiguous()
             o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if any(ctx.needs_input_grad[:3]) else None
+            stats = low = None
+            if any(ctx.needs_input_grad[:3]):
+                stats = torch.empty((2 if dtype == _lib.F32 else 1, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+                low = torch.empty_like(o) if dtype != _lib.F32 else None
             desc = ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype))
             n = ctypes.c_int64()
             check(L.sempyr_attention_workspace(desc, ctypes.byref(n)), "sempyr_attention_workspace")
             ws = _workspace(4 * n.value, q.device)
             check(L.sempyr_attention_fwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k),
-                                         o.data_ptr(), _p(lse), _p(ws), n.value, _stream()), "sempyr_attention_fwd")
-        if lse is not None:
-            ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k, len_k)
+                                         o.data_ptr(), _p(low), _p(stats), _p(ws), n.value, _stream()), "sempyr_attention_fwd")
+        if stats is not None:
+            ctx.save_for_backward(q, k, v, o, low, stats, cu_q, cu_k, len_k)
             ctx.cfg = (causal, scale, dtype)
         return o
 
     @staticmethod
     def backward(ctx, g):
         _no_second_order("attention", g)
-        q, k, v, o, lse, cu_q, cu_k, len_k = ctx.saved_tensors
+        q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
         causal, scale, dtype = ctx.cfg
         with _on_device(q.device):
             g = g.contiguous()
             g = g if g.data_ptr() % 16 == 0 else g.clone()
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            delta = torch.empty_like(lse)
+            delta = torch.empty_like(stats[0])
             check(L.sempyr_attention_bwd(ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype)), q.data_ptr(),
-                                         k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
+                                         k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
                                          cu_k.data_ptr(), _p(len_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                          delta.data_ptr(), _stream()), "sempyr_attention_bwd")
         return dq, dk, dv, None, None, None, None, None, None

@@ -142,18 +142,18 @@ def test_attention_c_entries_refuse():
         d = _lib.AttentionDesc(**{**good, **change})
         n = ctypes.c_int64()
         assert L.sempyr_attention_workspace(ctypes.byref(d), ctypes.byref(n)) < 0, change
-        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, 0, 16) < 0, change
-        assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 14) < 0, change
+        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 10, 0, 16) < 0, change
+        assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 15) < 0, change
     d = _lib.AttentionDesc(**good)
     for hole in (0, 1, 2, 3, 4, 6):                     # (5: len_k may be absent)
-        args = [16] * 9 + [0, 16]
+        args = [16] * 10 + [0, 16]
         args[hole] = 0
         assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0, hole
-    args = [16] * 9 + [0, 16]
+    args = [16] * 10 + [0, 16]
     args[1] = 20                                        # keys that are not 16-byte aligned
     assert L.sempyr_attention_fwd(ctypes.byref(d), *args) < 0
     n = ctypes.c_int64()
     d = _lib.AttentionDesc(**{**good, "total_q": 1, "total_k": 4096})
     assert L.sempyr_attention_workspace(ctypes.byref(d), ctypes.byref(n)) == 0 and n.value > 0
-    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, n.value - 1, 16) < 0 and b"workspace" in L.sempyr_last_error_string()
-    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 8, 0, n.value, 16) < 0
+    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 10, n.value - 1, 16) < 0 and b"workspace" in L.sempyr_last_error_string()
+    assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, 0, n.value, 16) < 0
