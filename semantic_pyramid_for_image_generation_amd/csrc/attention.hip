@@ -76,5 +76,5 @@ extern "C" int sempyr_attention_bwd(const sempyr_attention_desc* d, const void* 
     if ((int64_t)d->heads_q * d->dim > (int64_t)1 << 23) SEMPYR_FAIL("attention_bwd: rows of more than 2^23 elements");
     p.q = q; p.k = k; p.v = v; p.cu_q = cu_q; p.cu_k = cu_k; p.len_k = len_k;
     p.o = const_cast<void*>(o); p.o_low = const_cast<void*>(o_low); p.stats = const_cast<float*>(stats); p.go = go; p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
-    return attn::launch_bwd(d->dtype, p, delta, (hipStream_t)stream);
+    return attn::launch_bwd(d->dtype, p, (hipStream_t)stream);
 }

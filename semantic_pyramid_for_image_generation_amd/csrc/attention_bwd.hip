@@ -1,43 +1,13 @@
 // Backward of the packed attention.  With P recomputed from the forward's row statistics (see Stats):
 //     dV = P^T dO,  dP = dO V^T,  dS = P o (dP - delta),  delta = rowsum(dO o O),  dQ = scale dS K,  dK = scale dS^T Q
 // Two kernels without atomics, each owning what it sums, so the result does not depend on timing: one workgroup per 32 or 64
-// keys walks over the queries of all heads of its group (dK, dV), one per 128 queries walks over the keys (dQ).  That costs seven
+// keys walks over the queries of all heads of its group (dK, dV), one per 128 queries walks over the keys (delta, dQ; it runs
+// first).  That costs seven
 // products a tile pair instead of five; the two that are repeated are what the order of an atomic sum would otherwise cost.
 #include "attn_tile.h"
 #include "attention.h"
 
 namespace attn {
-
-constexpr int BM = 128, BN = 64;
-
-// delta[head][row] = sum over d of go * o, 16 lanes a row.  For 16-bit types o is taken with what its rounding left (o_low):
-// an error of delta is common to a row, so dQ would carry the rounding of o (2^-9 for bf16) in full.
-template <typename T>
-__global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restrict__ go, const T* __restrict__ o, const T* __restrict__ o_low,
-                                                              float* __restrict__ delta,
-                                                              int64_t rows, int total_q, int heads, int dim)
-{
-    constexpr int N = Vec16<T>::N;
-    const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    if (row >= rows) return;
-    float sum = 0.f;
-    for (int d = (threadIdx.x % 16) * N; d < dim; d += 16 * N) {
-        float a[N], b[N];
-        load_floats<T, N>(go + row * dim + d, a);
-        load_floats<T, N>(o + row * dim + d, b);
-        if (o_low) {
-            float c[N];
-            load_floats<T, N>(o_low + row * dim + d, c);
-#pragma unroll
-            for (int i = 0; i < N; ++i) b[i] += c[i];
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum = fmaf(a[i], b[i], sum);
-    }
-#pragma unroll
-    for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
-    if (threadIdx.x % 16 == 0) delta[(row % heads) * total_q + row / heads] = sum;
-}
 
 // dK, dV of 32 KB keys.  The steps of a workgroup -- tiles of 32 queries of every head of the group -- are dealt to its four
 // waves; a wave streams its tiles (Q, dO, row statistics) through an LDS ring of its own, so there is no barrier in the loop, and
@@ -46,14 +16,15 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const T* __restric
 // the LDS traffic that would otherwise bound the loop.  At the end the waves' sums are joined in LDS in wave order.
 template <typename T, int DPAD> struct KeyTile {
     typedef Tile<T, DPAD, 32> Tl;
-    static constexpr int KB = sizeof(T) * DPAD <= 256 ? 2 : 1, KEYS = 32 * KB;       // registers: 2 KB (fragments + sums) of DPAD columns
+    static constexpr int KB = sizeof(T) == 4 && DPAD <= 64 ? 2 : 1, KEYS = 32 * KB;
     static constexpr int WAVES = sizeof(T) * DPAD > 256 ? 2 : 4;        // two where four rings would not fit the LDS
     static constexpr int BUF = 2 * Tl::BYTES + (Stats<T>::N + 1) * 256, PAD = DPAD + 4;
-    static constexpr int RINGS = WAVES * 2 * BUF, JOIN = WAVES * KEYS * PAD * 4, LDS = RINGS > JOIN ? RINGS : JOIN;
+    static constexpr int STAGES = 2, LOADS = 2 * Tl::LOADS + 1 + Stats<T>::N;
+    static constexpr int RINGS = WAVES * STAGES * BUF, JOIN = WAVES * KEYS * PAD * 4, LDS = RINGS > JOIN ? RINGS : JOIN;
 };
 
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
+__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 128 ? 2 : 1) void attention_dkdv_kernel(Params p)
 {
     typedef KeyTile<T, DPAD> Kt;
     typedef Tile<T, DPAD, 32> Tl;
@@ -81,13 +52,22 @@ __global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
 
     // query tiles that see any of the keys
     const int first = p.causal ? max(0, row0 - shift) / 32 : 0;
-    const int ntiles = row0 < sq.lk ? max(0, (sq.lq + 31) / 32 - first) : 0, steps = ntiles * p.group;
+    const int ntiles = row0 < sq.lk ? max(0, (sq.lq + 31) / 32 - first) : 0;
     Filler<T, DPAD, 32, 1> fq, fo;
     fq.init(p.q_tok, p.dim, 0, lane);
     fo.init((int64_t)p.heads_q * p.dim, p.dim, 0, lane);
-    char* ring = lds + wave * 2 * Kt::BUF;
-    auto fill = [&](int it, int b) {
-        const int head = w.kvh * p.group + it / ntiles, r = (first + it % ntiles) * 32, left = sq.lq - r;
+    char* ring = lds + wave * Kt::STAGES * Kt::BUF;
+    // a wave's steps: head g of the group and tile t of it, counted from the sequence's end: workgroups of one sequence start on
+    // the same tiles whatever their diagonal, and find them in L2
+    struct Step { int g, t; };
+    auto advance = [&](Step s) {
+        s.t += WAVES;
+        while (s.t >= ntiles) { s.t -= ntiles; ++s.g; }
+        return s;
+    };
+    auto fill = [&](Step s, int b) {                  // behind the last step: zeros, so that the loop's waits stay the same
+        const bool more = s.g < p.group;
+        const int r = (first + ntiles - 1 - s.t) * 32, head = w.kvh * p.group + (more ? s.g : 0), left = more ? sq.lq - r : 0;
         const int64_t row = sq.q0 + r;
         char* buf = ring + b * Kt::BUF;
         fq.issue((const T*)p.q + row * p.q_tok + (int64_t)head * p.q_head, left, buf);
@@ -104,17 +84,19 @@ __global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
         }
     };
     const int rbase = Tl::row_base(lane), cbase = Tl::col_base(lane);
-    if (wave < steps) fill(wave, 0);
+    Step cur = {0, wave - WAVES}, next = cur;
+    if (ntiles > 0) {
+        next = cur = advance(cur);
+#pragma unroll
+        for (int u = 0; u < Kt::STAGES - 1; ++u) { fill(next, u); next = advance(next); }
+    }
     int b = 0;
-    for (int it = wave; it < steps; it += WAVES, b ^= 1) {
-        if (it + WAVES < steps) {
-            wait_lds();
-            fill(it + WAVES, b ^ 1);
-            wait_loads<2 * Tl::LOADS + 1 + Stats<T>::N>();
-        } else {
-            wait_loads<0>();
-        }
-        const int qb = (first + it % ntiles) * 32;
+    for (; ntiles > 0 && cur.g < p.group; cur = advance(cur), b = b + 1 == Kt::STAGES ? 0 : b + 1) {
+        wait_lds();                                   // the buffer filled next was read in the step before
+        fill(next, b == 0 ? Kt::STAGES - 1 : b - 1);
+        next = advance(next);
+        wait_loads<(Kt::STAGES - 1) * Kt::LOADS>();
+        const int qb = (first + ntiles - 1 - cur.t) * 32;
         const char *qt = ring + b * Kt::BUF, *ot = qt + Tl::BYTES;
         const float *delta = reinterpret_cast<const float*>(ot + Tl::BYTES), *ref = delta + 64, *inv = ref + 64;
         f32x16 sc[KB], dp[KB];
@@ -155,24 +137,43 @@ __global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
                 for (int i = 0; i < 16; ++i)
                     if (row0 + n * 32 + (lane & 31) > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[n][i] = dp[n][i] = 0.f;
         }
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            Frag pf[KB], df[KB];
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int n = 0; n < KB; ++n) { pf[n] = frag_of<T>(sc[n], k); df[n] = frag_of<T>(dp[n], k); }
+                for (int c = 0; c < DPAD / 32; ++c) {
+                    const Frag fo_ = Tl::col(ot, cbase, c, k), fq_ = Tl::col(qt, cbase, c, k);
 #pragma unroll
-            for (int c = 0; c < DPAD / 32; ++c) {
-                const Frag fo_ = Tl::col(ot, cbase, c, k), fq_ = Tl::col(qt, cbase, c, k);
+                    for (int n = 0; n < KB; ++n) {
+                        dv[n][c] = Elem<T>::mma(fo_, frag_of<T>(sc[n], k), dv[n][c]);
+                        dk[n][c] = Elem<T>::mma(fq_, frag_of<T>(dp[n], k), dk[n][c]);
+                    }
+                }
+        } else {
+            Frag x[2][DPAD / 32];
+            Tl::template cols<0>(x, ot, cbase);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int n = 0; n < KB; ++n) {
-                    dv[n][c] = Elem<T>::mma(fo_, pf[n], dv[n][c]);
-                    dk[n][c] = Elem<T>::mma(fq_, df[n], dk[n][c]);
+                    const Frag pf = frag_of<T>(sc[n], k);
+#pragma unroll
+                    for (int c = 0; c < DPAD / 32; ++c) dv[n][c] = Elem<T>::mma(x[k][c], pf, dv[n][c]);
                 }
-            }
+            Tl::template cols<0>(x, qt, cbase);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int n = 0; n < KB; ++n) {
+                    const Frag df = frag_of<T>(dp[n], k);
+#pragma unroll
+                    for (int c = 0; c < DPAD / 32; ++c) dk[n][c] = Elem<T>::mma(x[k][c], df, dk[n][c]);
+                }
         }
     }
 
     // join: [wave][key][dim] fp32 in LDS, dV first, then dK
+    wait_loads<0>();
     float* joined = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -201,13 +202,14 @@ __global__ __launch_bounds__(256, 1) void attention_dkdv_kernel(Params p)
     }
 }
 
-// dQ: as the forward, with dO beside Q in registers and K read by columns, too.
+// delta and dQ: as the forward, with dO beside Q in registers and K read by columns, too.
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(Params p)
+__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attention_dq_kernel(Params p)
 {
     typedef Tile<T, DPAD, BN> Tl;
     typedef typename Elem<T>::Frag Frag;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // [2 buffers][K tile, V tile]
+    constexpr int STAGES = stages_of<T, DPAD>();
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [buffer][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Work w = work_of(blockIdx.x, p.heads_k, p.group);
     const Where at = locate<false>(p, w.number, BM, lane);
@@ -223,7 +225,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     load_row_frags<T, DPAD>(qf, (const T*)p.q + (int64_t)(sq.q0 + qi) * p.q_tok + (int64_t)head * p.q_head, present, p.dim, lane);
     load_row_frags<T, DPAD>(of, (const T*)p.go + orow, present, p.dim, lane);
     const int64_t stat = (int64_t)head * p.total_q + sq.q0 + qi;
-    const float ref = present ? p.stats[stat] : INFINITY, delta = present ? p.delta[stat] : 0.f;
+    const float ref = present ? p.stats[stat] : INFINITY;
+    // delta = rowsum(dO o O), kept for the other kernel.  For 16-bit types O is taken with what its rounding left (o_low): an
+    // error of delta is common to a row, dQ would carry the rounding of O (2^-9 for bf16) in full.
+    float delta = 0.f;
+    {
+        Frag x[DPAD / 16];
+        load_row_frags<T, DPAD>(x, (const T*)p.o + orow, present, p.dim, lane);
+#pragma unroll
+        for (int d = 0; d < DPAD / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta = fmaf((float)x[d][i], (float)of[d][i], delta);
+        if (sizeof(T) == 2 && p.o_low) {
+            load_row_frags<T, DPAD>(x, (const T*)p.o_low + orow, present, p.dim, lane);
+#pragma unroll
+            for (int d = 0; d < DPAD / 16; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) delta = fmaf((float)x[d][i], (float)of[d][i], delta);
+        }
+        delta = half_sum(delta);
+        if (present && half == 0) p.delta[stat] = delta;
+    }
 
     const int see = p.causal ? min(sq.lk, qi + 1 + shift) : sq.lk;
     const int see_first = p.causal ? min(sq.lk, row0 + wave * 32 + 1 + shift) : sq.lk;
@@ -236,35 +258,43 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     fv.init(p.v_tok, p.dim, wave, lane);
     const T* kbase = (const T*)p.k + (int64_t)sq.k0 * p.k_tok + (int64_t)w.kvh * p.k_head;
     const T* vbase = (const T*)p.v + (int64_t)sq.k0 * p.v_tok + (int64_t)w.kvh * p.v_head;
-    auto fill = [&](int t) {
-        char* buf = lds + (t & 1) * 2 * Tl::BYTES;
-        fk.issue(kbase + (int64_t)t * BN * p.k_tok, sq.lk - t * BN, buf);
-        fv.issue(vbase + (int64_t)t * BN * p.v_tok, sq.lk - t * BN, buf + Tl::BYTES);
+    auto fill = [&](int t, int b) {                   // behind the last tile: zeros, so that the loop's waits stay the same
+        char* buf = lds + b * 2 * Tl::BYTES;
+        const int left = t < tiles ? sq.lk - t * BN : 0, at = t < tiles ? t * BN : 0;
+        fk.issue(kbase + (int64_t)at * p.k_tok, left, buf);
+        fv.issue(vbase + (int64_t)at * p.v_tok, left, buf + Tl::BYTES);
     };
     const int rbase = Tl::row_base(lane), cbase = Tl::col_base(lane);
     f32x16 acc[DPAD / 32];
 #pragma unroll
     for (int b = 0; b < DPAD / 32; ++b) acc[b] = f32x16{};
-    if (tiles) fill(0);
-    for (int t = 0; t < tiles; ++t) {
-        wait_loads<0>();
-        barrier();
-        if (t + 1 < tiles) fill(t + 1);
+    if (tiles) {
+#pragma unroll
+        for (int u = 0; u < STAGES - 1; ++u) fill(u, u);
+    }
+    int b = 0;
+    for (int t = 0; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+        wait_loads<(STAGES - 2) * 2 * Filler<T, DPAD, BN, 4>::N>();
+        barrier();                                   // tile t is complete, nobody reads the buffer of tile t - 1 any more
+        fill(t + STAGES - 1, b == 0 ? STAGES - 1 : b - 1);
         const int key0 = t * BN;
         if (key0 >= see_wave) continue;
-        const char *kt = lds + (t & 1) * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
+        const char *kt = lds + b * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
         const bool edge = key0 + BN > see_first;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int n = 0; n < 2; ++n) {
             f32x16 sc = f32x16{}, dp = f32x16{};
 #pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) sc = Elem<T>::mma(Tl::row(kt, rbase, b, d), qf[d], sc);
+            for (int d = 0; d < DPAD / 16; ++d) sc = Elem<T>::mma(Tl::row(kt, rbase, n, d), qf[d], sc);
 #pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) dp = Elem<T>::mma(Tl::row(vt, rbase, b, d), of[d], dp);
+            for (int d = 0; d < DPAD / 16; ++d) dp = Elem<T>::mma(Tl::row(vt, rbase, n, d), of[d], dp);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool hidden = edge && key0 + b * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see;
-                dp[i] = hidden ? 0.f : score_exp<T>(sc[i], p.scale_log2, ref) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i)
+                dp[i] = score_exp<T>(sc[i], p.scale_log2, ref) * (dp[i] - delta);
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + n * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see) dp[i] = 0.f;
             }
             if constexpr (sizeof(T) == 4) {
                 // 32 keys are summed by themselves first, see the forward
@@ -272,19 +302,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
                 for (int c = 0; c < DPAD / 32; ++c) {
                     f32x16 part = f32x16{};
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) part = Elem<T>::mma(Tl::col(kt, cbase, c, b * 2 + k), frag_of<T>(dp, k), part);
+                    for (int k = 0; k < 2; ++k) part = Elem<T>::mma(Tl::col(kt, cbase, c, n * 2 + k), frag_of<T>(dp, k), part);
                     acc[c] += part;
                 }
             } else {
+                Frag x[2][DPAD / 32];
+                n == 0 ? Tl::template cols<0>(x, kt, cbase) : Tl::template cols<2>(x, kt, cbase);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const Frag df = frag_of<T>(dp, k);
 #pragma unroll
-                    for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(kt, cbase, c, b * 2 + k), df, acc[c]);
+                    for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(x[k][c], df, acc[c]);
                 }
             }
         }
     }
+    wait_loads<0>();
     if (!present) return;
     float f = p.scale;
     if (sizeof(T) == 4) f *= p.stats[(int64_t)p.heads_q * p.total_q + stat];
@@ -311,37 +344,31 @@ static int launch_bwd_d(const Params& p, hipStream_t st) {
     const int64_t bk = work_blocks(num_tiles(p.nseq, p.total_k, Kt::KEYS), p.heads_k, 1);
     const int64_t bq = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
     if (bk > 0x7FFFFFFF || bq > 0x7FFFFFFF) SEMPYR_FAIL("attention_bwd: too many tiles");
-    const int lds_q = 4 * Tile<T, DPAD, BN>::BYTES;
-    if (p.total_k > 0) {
-        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, Kt::LDS)) return rc;
-        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 64 * Kt::WAVES, Kt::LDS, st>>>(p);
-        SEMPYR_CHECK_LAUNCH();
-    }
+    const int lds_q = stages_of<T, DPAD>() * 2 * Tile<T, DPAD, BN>::BYTES;
     if (p.total_q > 0) {
         if (int rc = allow_lds((const void*)attention_dq_kernel<T, DPAD>, lds_q)) return rc;
         attention_dq_kernel<T, DPAD><<<(unsigned)bq, 256, lds_q, st>>>(p);
+        SEMPYR_CHECK_LAUNCH();
+    }
+    if (p.total_k > 0) {
+        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, Kt::LDS)) return rc;
+        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 64 * Kt::WAVES, Kt::LDS, st>>>(p);
         SEMPYR_CHECK_LAUNCH();
     }
     return 0;
 }
 
 template <typename T>
-static int launch_bwd_t(const Params& p, float* delta, hipStream_t st) {
-    const int64_t rows = (int64_t)p.total_q * p.heads_q;
-    if (rows > 0) {
-        if (rows > 0x7FFFFFFFll * 16) SEMPYR_FAIL("attention_bwd: too many rows");
-        attention_delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>((const T*)p.go, (const T*)p.o, (const T*)p.o_low, delta, rows, p.total_q, p.heads_q, p.dim);
-        SEMPYR_CHECK_LAUNCH();
-    }
+static int launch_bwd_t(const Params& p, hipStream_t st) {
     if (p.dim <= 32) return launch_bwd_d<T, 32>(p, st);
     if (p.dim <= 64) return launch_bwd_d<T, 64>(p, st);
     return launch_bwd_d<T, 128>(p, st);
 }
 
-int launch_bwd(int dtype, const Params& p, float* delta, hipStream_t st) {
-    if (dtype == SEMPYR_F32) return launch_bwd_t<float>(p, delta, st);
-    if (dtype == SEMPYR_F16) return launch_bwd_t<f16>(p, delta, st);
-    return launch_bwd_t<bf16>(p, delta, st);
+int launch_bwd(int dtype, const Params& p, hipStream_t st) {
+    if (dtype == SEMPYR_F32) return launch_bwd_t<float>(p, st);
+    if (dtype == SEMPYR_F16) return launch_bwd_t<f16>(p, st);
+    return launch_bwd_t<bf16>(p, st);
 }
 
 }  // namespace attn

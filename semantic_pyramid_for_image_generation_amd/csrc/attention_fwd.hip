@@ -1,22 +1,22 @@
 // Forward of the packed attention: O = softmax(scale Q K^T + mask) V in one pass over the keys with a running maximum and sum.
 //
 // A workgroup owns 128 queries of one head, a wave 32 of them (a query = a lane pair, see attn_tile.h).  Per tile of 64 keys:
-//     S^T = K Q^T, running maximum m, P = exp2(c S - c m), l += sum P, O^T = O^T exp2(c (m_old - m)) + V^T P
-// with c = scale log2(e).  Queries and the output accumulator stay in registers; K and V tiles are double-buffered in LDS, the
-// next tile's DMA runs under the current tile's products.
+//     S^T = K Q^T, P = exp2(c S - c m), l += sum P, O^T += V^T P
+// with c = scale log2(e) and a reference m that follows the maximum in steps (l and O^T are rescaled when it moves).  Queries and the output accumulator stay in registers; K and V tiles come through a ring in
+// LDS, the next tiles' DMA runs under the current tile's products.
 #include "attn_tile.h"
 #include "attention.h"
 
 namespace attn {
 
-constexpr int BM = 128, BN = 64;
 
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
+__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attention_fwd_kernel(Params p)
 {
     typedef Tile<T, DPAD, BN> Tl;
     typedef typename Elem<T>::Frag Frag;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // [2 buffers][K tile, V tile]
+    constexpr int STAGES = stages_of<T, DPAD>();
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [buffer][K tile, V tile]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Work w = work_of(blockIdx.x, p.heads_k, p.group);
     const Where at = locate<false>(p, w.number, BM, lane);
@@ -42,25 +42,30 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
     fv.init(p.v_tok, p.dim, wave, lane);
     const T* kbase = (const T*)p.k + (int64_t)sq.k0 * p.k_tok + (int64_t)w.kvh * p.k_head;
     const T* vbase = (const T*)p.v + (int64_t)sq.k0 * p.v_tok + (int64_t)w.kvh * p.v_head;
-    auto fill = [&](int t) {
-        char* buf = lds + (t & 1) * 2 * Tl::BYTES;
-        fk.issue(kbase + (int64_t)t * BN * p.k_tok, sq.lk - t * BN, buf);
-        fv.issue(vbase + (int64_t)t * BN * p.v_tok, sq.lk - t * BN, buf + Tl::BYTES);
+    auto fill = [&](int t, int b) {                   // behind the last tile: zeros, so that the loop's waits stay the same
+        char* buf = lds + b * 2 * Tl::BYTES;
+        const int left = t < tiles ? sq.lk - t * BN : 0, at = t < tiles ? t * BN : 0;
+        fk.issue(kbase + (int64_t)at * p.k_tok, left, buf);
+        fv.issue(vbase + (int64_t)at * p.v_tok, left, buf + Tl::BYTES);
     };
     const int rbase = Tl::row_base(lane), cbase = Tl::col_base(lane);
 
     f32x16 acc[DPAD / 32];
 #pragma unroll
     for (int b = 0; b < DPAD / 32; ++b) acc[b] = f32x16{};
-    float m = -INFINITY, l = 0.f;
-    if (tiles) fill(0);
-    for (int t = 0; t < tiles; ++t) {
-        wait_loads<0>();
-        barrier();                                   // tile t is complete, nobody reads the other buffer any more
-        if (t + 1 < tiles) fill(t + 1);
+    float m = -INFINITY, base = 0.f, l = 0.f;            // reference, see REF_SLACK; its form for the exponential; sum
+    if (tiles) {
+#pragma unroll
+        for (int u = 0; u < STAGES - 1; ++u) fill(u, u);
+    }
+    int b = 0;
+    for (int t = 0; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+        wait_loads<(STAGES - 2) * 2 * Filler<T, DPAD, BN, 4>::N>();
+        barrier();                                   // tile t is complete, nobody reads the buffer of tile t - 1 any more
+        fill(t + STAGES - 1, b == 0 ? STAGES - 1 : b - 1);
         const int key0 = t * BN;
         if (key0 >= see_wave) continue;              // above the diagonal for all of this wave's queries
-        const char *kt = lds + (t & 1) * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
+        const char *kt = lds + b * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
         f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -73,15 +78,23 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
                 for (int i = 0; i < 16; ++i)
                     if (key0 + b * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see) sc[b][i] = -INFINITY;
         }
-        float mx = m;
+        float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float base = score_ref<T>(mx, p.scale_log2);                  // 0 for a row that has seen no key yet
-        const float alpha = score_exp<T>(m, p.scale_log2, base);
-        m = mx;
+        mx = half_max(mx);
+        if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {                // (never for NaN; a row without a key: -inf > slack)
+            const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
+            const float alpha = score_exp<T>(m, p.scale_log2, moved);
+            m = top;
+            base = moved;
+            l *= alpha;
+#pragma unroll
+            for (int b = 0; b < DPAD / 32; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -90,7 +103,7 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
                 sc[b][i] = score_exp<T>(sc[b][i], p.scale_log2, base);
                 sum += sc[b][i];
             }
-        l = l * alpha + sum;
+        l += sum;
         if constexpr (sizeof(T) == 4) {
             // a tile's products are summed by themselves first: a chain over all keys would lose bits with its length
 #pragma unroll
@@ -99,22 +112,26 @@ __global__ __launch_bounds__(256, 2) void attention_fwd_kernel(Params p)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) part = Elem<T>::mma(Tl::col(vt, cbase, b, k), frag_of<T>(sc[k / 2], k % 2), part);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][i] = fmaf(acc[b][i], alpha, part[i]);
+                for (int i = 0; i < 16; ++i) acc[b][i] += part[i];
             }
         } else {
+            Frag vf[2][DPAD / 32];
+            auto products = [&](const f32x16& x) {
 #pragma unroll
-            for (int b = 0; b < DPAD / 32; ++b)
+                for (int k = 0; k < 2; ++k) {
+                    const Frag pf = frag_of<T>(x, k);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const Frag pf = frag_of<T>(sc[k / 2], k % 2);
-#pragma unroll
-                for (int b = 0; b < DPAD / 32; ++b) acc[b] = Elem<T>::mma(Tl::col(vt, cbase, b, k), pf, acc[b]);
-            }
+                    for (int b = 0; b < DPAD / 32; ++b) acc[b] = Elem<T>::mma(vf[k][b], pf, acc[b]);
+                }
+            };
+            Tl::template cols<0>(vf, vt, cbase);
+            products(sc[0]);
+            Tl::template cols<2>(vf, vt, cbase);
+            products(sc[1]);
         }
     }
-    l += __shfl_xor(l, 32, 64);                      // each lane half has summed its own keys
+    wait_loads<0>();
+    l = half_sum(l);                                 // each lane half has summed its own keys
     if (!present) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;      // no key: zeros
     const int64_t out = ((int64_t)(sq.q0 + qi) * p.heads_q + head) * p.dim;
@@ -132,7 +149,7 @@ template <typename T, int DPAD>
 static int launch_fwd_d(const Params& p, hipStream_t st) {
     const int64_t blocks = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
     if (blocks > 0x7FFFFFFF) SEMPYR_FAIL("attention_fwd: too many tiles");
-    const int bytes = 4 * Tile<T, DPAD, BN>::BYTES;
+    const int bytes = stages_of<T, DPAD>() * 2 * Tile<T, DPAD, BN>::BYTES;
     if (int rc = allow_lds((const void*)attention_fwd_kernel<T, DPAD>, bytes)) return rc;
     attention_fwd_kernel<T, DPAD><<<(unsigned)blocks, 256, bytes, st>>>(p);
     SEMPYR_CHECK_LAUNCH();

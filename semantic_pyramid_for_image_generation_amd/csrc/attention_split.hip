@@ -79,7 +79,7 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
     f32x16 acc[DPAD / 32];
 #pragma unroll
     for (int b = 0; b < DPAD / 32; ++b) acc[b] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, base = 0.f, l = 0.f;
     if (t0 < t1) fill(t0, 0);
     int b = 0;
     for (int t = t0; t < t1; t += WAVES, b ^= 1) {
@@ -100,32 +100,47 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
             for (int i = 0; i < 16; ++i)
                 if (key0 + (i / 4) * 8 + half * 4 + i % 4 >= see) sc[i] = -INFINITY;
         }
-        float mx = m;
+        float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float base = score_ref<T>(mx, p.scale_log2);
-        const float alpha = score_exp<T>(m, p.scale_log2, base);
-        m = mx;
+        mx = half_max(mx);
+        if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {
+            const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
+            const float alpha = score_exp<T>(m, p.scale_log2, moved);
+            m = top;
+            base = moved;
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < DPAD / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c][i] *= alpha;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             sc[i] = score_exp<T>(sc[i], p.scale_log2, base);
             sum += sc[i];
         }
-        l = l * alpha + sum;
+        l += sum;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int c = 0; c < DPAD / 32; ++c)
+            for (int k = 0; k < 2; ++k) {
+                const Frag pf = frag_of<T>(sc, k);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c][i] *= alpha;
+                for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(vt, cbase, c, k), pf, acc[c]);
+            }
+        } else {
+            Frag vf[2][DPAD / 32];
+            Tl::template cols<0>(vf, vt, cbase);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const Frag pf = frag_of<T>(sc, k);
+            for (int k = 0; k < 2; ++k) {
+                const Frag pf = frag_of<T>(sc, k);
 #pragma unroll
-            for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(vt, cbase, c, k), pf, acc[c]);
+                for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(vf[k][c], pf, acc[c]);
+            }
         }
     }
-    l += __shfl_xor(l, 32, 64);
+    l = half_sum(l);
 
     // join the waves: [wave][column][dim] in LDS, every thread then owns four elements of a column
     wait_lds();

@@ -30,7 +30,7 @@ struct Params {
     void* o_low;                                             // 16-bit types: what rounding took from o, for delta; or null
     float* stats;                                            // rows' softmax statistics for the backward pass (see Stats), or null
     const void* go;                                          // backward: gradient of o, contiguous
-    const float* delta;                                      // backward: [heads_q][total_q] rowsum(go * o)
+    float* delta;                                            // backward: [heads_q][total_q] rowsum(go * o)
     void *dq, *dk, *dv;                                      // backward: contiguous
     const int32_t *cu_q, *cu_k, *len_k;
     int total_q, total_k, nseq, heads_q, heads_k, group, dim, causal;
@@ -101,27 +101,54 @@ struct Tile {
         }
         return h * 4 * ROWB + (((lane & 31) >> 2 ^ swz(h * 4)) << 4) + (lane & 3) * 4;
     }
-    // column 32 block + lane % 32, rows 16 t + 8 (j / 4) + 4 h + j % 4
+    // fp32: column 32 block + lane % 32, rows 16 t + 8 (j / 4) + 4 h + j % 4
     static __device__ __forceinline__ Frag col(const char* tile, int base, int block, int t) {
+        static_assert(SZ == 4, "16-bit types read their columns with cols()");
         Frag f;
-        if constexpr (SZ == 2) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const char* p = tile + (t * 16 + u * 8) * ROWB + (base ^ block * 64 ^ u * 32);
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR s16x4*)(p));
-                typedef T V4 __attribute__((ext_vector_type(4)));
-                const V4 y = __builtin_bit_cast(V4, x);      // (as a whole: the cast of one vector element takes element 0)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[u * 4 + j] = y[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int r = (j / 4) * 8 + j % 4;
-                f[j] = *reinterpret_cast<const float*>(tile + (t * 16 + r) * ROWB + (base ^ block * 128 ^ swz(r) << 4));
-            }
+        for (int j = 0; j < 8; ++j) {
+            const int r = (j / 4) * 8 + j % 4;
+            f[j] = *reinterpret_cast<const float*>(tile + (t * 16 + r) * ROWB + (base ^ block * 128 ^ swz(r) << 4));
         }
         return f;
+    }
+    // 16-bit types: the same of groups T and T + 1 for all column blocks, f[group][block].  Written in assembly because the
+    // compiler puts a wait for ALL vector memory before the builtin of a transposing read, also for the DMA that fills other
+    // buffers; the reads' own wait is part of the block.
+    template <int T0>
+    static __device__ __forceinline__ void cols(Frag (&f)[2][DPAD / 32], const char* tile, int base) {
+        static_assert(SZ == 2, "fp32 reads its columns with col()");
+        constexpr int O = T0 * 16 * ROWB, G = 16 * ROWB, H = 8 * ROWB;      // first group; next group; second half of a group
+        const unsigned at = (unsigned)(uintptr_t)(LDS_PTR const char*)tile;
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        if constexpr (DPAD == 32) {
+            s16x4 x[4];
+            asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%7\n\t"
+                         "ds_read_b64_tr_b16 %2, %4 offset:%8\n\tds_read_b64_tr_b16 %3, %5 offset:%9\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+                         : "v"(at + base), "v"(at + (base ^ 32)), "n"(O), "n"(O + H), "n"(O + G), "n"(O + G + H) : "memory");
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                f[g][0] = __builtin_shufflevector(__builtin_bit_cast(V4, x[2 * g]), __builtin_bit_cast(V4, x[2 * g + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+#pragma unroll
+            for (int c = 0; c < DPAD / 32; c += 2) {
+                s16x4 x[8];                               // [group][block][half]
+                asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%13\n\t"
+                             "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%13\n\t"
+                             "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %5, %9 offset:%15\n\t"
+                             "ds_read_b64_tr_b16 %6, %10 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                             : "v"(at + (base ^ c * 64)), "v"(at + (base ^ c * 64 ^ 32)), "v"(at + (base ^ (c + 1) * 64)),
+                               "v"(at + (base ^ (c + 1) * 64 ^ 32)), "n"(O), "n"(O + H), "n"(O + G), "n"(O + G + H) : "memory");
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        f[g][c + u] = __builtin_shufflevector(__builtin_bit_cast(V4, x[g * 4 + u * 2]), __builtin_bit_cast(V4, x[g * 4 + u * 2 + 1]),
+                                                              0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        }
     }
 };
 
@@ -182,6 +209,16 @@ __device__ __forceinline__ void load_row_frags(typename Elem<T>::Frag* f, const 
     }
 }
 
+// x of the other lane half, combined: gfx950 swaps the halves in the vector unit, no LDS round trip
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // 4 consecutive elements
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
@@ -210,6 +247,9 @@ __device__ __forceinline__ float score_exp(float s, float c, float x) {
 }
 template <typename T>
 __device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c; }
+// The reference of a row (its maximum at some tile) moves only when a score passes it by this many powers of two: until then
+// exponentials are at most 2^8, which every type and the fp32 sums hold, and the sums need no rescaling.  fp32: always.
+template <typename T> constexpr float REF_SLACK = sizeof(T) == 4 ? 0.f : 8.f;
 
 // 4 consecutive elements of the output and, where it is asked for, of what their rounding left
 template <typename T>
