@@ -9,62 +9,62 @@
 
 namespace attn {
 
-// dK, dV of 32 KB keys.  The steps of a workgroup -- tiles of 32 queries of every head of the group -- are dealt to its four
-// waves; a wave streams its tiles (Q, dO, row statistics) through an LDS ring of its own, so there is no barrier in the loop, and
-// reads each by rows (scores, dP) and by columns (the two gradients).  K and V fragments and both gradients of all the keys
-// stay in registers: with KB = 2 every fragment that is read from LDS feeds two products (one for each 32 keys), which halves
-// the LDS traffic that would otherwise bound the loop.  At the end the waves' sums are joined in LDS in wave order.
+// dK, dV of 32 SHARE keys: a lane pair is a key, its K and V fragments and both gradients stay in registers.  The steps of a
+// workgroup -- tiles of 32 queries of every head of the group -- are dealt to GROUPS groups of SHARE waves, which divides the
+// longest workgroup's walk.  The waves of a group hold different keys and share its tiles (Q, dO, row statistics), each of
+// which is read by rows (scores, dP) and by columns (the two gradients).  At the end the groups' sums are joined in LDS.
+// 16-bit types: a ring for every wave, no barrier in the loop (packed batch of 16 692 tokens, 16/4 heads of 64, causal, bf16:
+// 237 us, in pairs 280: there the longest walk counts).  fp32: pairs, whose rings leave room for two waves a SIMD (16 x 1024
+// tokens, 2 heads of 64: 155 us, alone 173).
 template <typename T, int DPAD> struct KeyTile {
     typedef Tile<T, DPAD, 32> Tl;
-    static constexpr int KB = sizeof(T) == 4 && DPAD <= 64 ? 2 : 1, KEYS = 32 * KB;
-    static constexpr int WAVES = sizeof(T) * DPAD > 256 ? 2 : 4;        // two where four rings would not fit the LDS
+    static constexpr int SHARE = sizeof(T) == 4 ? 2 : 1, GROUPS = 4 / SHARE, KEYS = 32 * SHARE, STAGES = 2;
     static constexpr int BUF = 2 * Tl::BYTES + (Stats<T>::N + 1) * 256, PAD = DPAD + 4;
-    static constexpr int STAGES = 2, LOADS = 2 * Tl::LOADS + 1 + Stats<T>::N;
-    static constexpr int RINGS = WAVES * STAGES * BUF, JOIN = WAVES * KEYS * PAD * 4, LDS = RINGS > JOIN ? RINGS : JOIN;
+    static constexpr int RINGS = GROUPS * STAGES * BUF, JOIN = GROUPS * KEYS * PAD * 4, LDS = RINGS > JOIN ? RINGS : JOIN;
+    static constexpr int WAVES_SIMD = DPAD <= 64 ? 2 : 1;               // by registers: heads of 128 need more than 256
 };
 
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 128 ? 2 : 1) void attention_dkdv_kernel(Params p)
+__global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD((KeyTile<T, DPAD>::WAVES_SIMD)) void attention_dkdv_kernel(Params p)
 {
     typedef KeyTile<T, DPAD> Kt;
     typedef Tile<T, DPAD, 32> Tl;
     typedef typename Elem<T>::Frag Frag;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    constexpr int KB = Kt::KB, KEYS = Kt::KEYS, WAVES = Kt::WAVES;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // [wave][2 buffers][Q tile, dO tile, delta, statistics]
+    constexpr int KEYS = Kt::KEYS, STAGES = Kt::STAGES, SHARE = Kt::SHARE, GROUPS = Kt::GROUPS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [group][buffer][Q tile, dO tile, delta, statistics]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int group = wave / SHARE, member = wave % SHARE;
     const Work w = work_of(blockIdx.x, p.heads_k, 1);
     const Where where = locate<true>(p, w.number, KEYS, lane);
     if (!where.ok) return;
     const Seq sq = where.sq;
     const int row0 = where.row, shift = sq.lk - sq.lq;                    // first key within the sequence
+    const int kw0 = row0 + member * 32, ki = kw0 + (lane & 31);
 
-    Frag kf[KB][DPAD / 16], vf[KB][DPAD / 16];
-    f32x16 dk[KB][DPAD / 32], dv[KB][DPAD / 32];
+    Frag kf[DPAD / 16], vf[DPAD / 16];
+    load_row_frags<T, DPAD>(kf, (const T*)p.k + (int64_t)(sq.k0 + ki) * p.k_tok + (int64_t)w.kvh * p.k_head, ki < sq.lk, p.dim, lane);
+    load_row_frags<T, DPAD>(vf, (const T*)p.v + (int64_t)(sq.k0 + ki) * p.v_tok + (int64_t)w.kvh * p.v_head, ki < sq.lk, p.dim, lane);
+    settle(kf);
+    settle(vf);
+    f32x16 dk[DPAD / 32], dv[DPAD / 32];
 #pragma unroll
-    for (int n = 0; n < KB; ++n) {
-        const int ki = row0 + n * 32 + (lane & 31);
-        load_row_frags<T, DPAD>(kf[n], (const T*)p.k + (int64_t)(sq.k0 + ki) * p.k_tok + (int64_t)w.kvh * p.k_head, ki < sq.lk, p.dim, lane);
-        load_row_frags<T, DPAD>(vf[n], (const T*)p.v + (int64_t)(sq.k0 + ki) * p.v_tok + (int64_t)w.kvh * p.v_head, ki < sq.lk, p.dim, lane);
-#pragma unroll
-        for (int c = 0; c < DPAD / 32; ++c) dk[n][c] = dv[n][c] = f32x16{};
-    }
+    for (int c = 0; c < DPAD / 32; ++c) dk[c] = dv[c] = f32x16{};
 
-    // query tiles that see any of the keys
+    // query tiles that see any of the keys; a group's steps: head g and tile t of it, counted from the
+    // sequence's end
     const int first = p.causal ? max(0, row0 - shift) / 32 : 0;
     const int ntiles = row0 < sq.lk ? max(0, (sq.lq + 31) / 32 - first) : 0;
-    Filler<T, DPAD, 32, 1> fq, fo;
-    fq.init(p.q_tok, p.dim, 0, lane);
-    fo.init((int64_t)p.heads_q * p.dim, p.dim, 0, lane);
-    char* ring = lds + wave * Kt::STAGES * Kt::BUF;
-    // a wave's steps: head g of the group and tile t of it, counted from the sequence's end: workgroups of one sequence start on
-    // the same tiles whatever their diagonal, and find them in L2
     struct Step { int g, t; };
-    auto advance = [&](Step s) {
-        s.t += WAVES;
+    auto advance = [&](Step s, int by) {
+        s.t += by;
         while (s.t >= ntiles) { s.t -= ntiles; ++s.g; }
         return s;
     };
+    Filler<T, DPAD, 32, SHARE> fq, fo;
+    fq.init(p.q_tok, p.dim, member, lane);
+    fo.init((int64_t)p.heads_q * p.dim, p.dim, member, lane);
+    char* ring = lds + group * STAGES * Kt::BUF;
     auto fill = [&](Step s, int b) {                  // behind the last step: zeros, so that the loop's waits stay the same
         const bool more = s.g < p.group;
         const int r = (first + ntiles - 1 - s.t) * 32, head = w.kvh * p.group + (more ? s.g : 0), left = more ? sq.lq - r : 0;
@@ -72,139 +72,102 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 128 ? 2 : 1) void attentio
         char* buf = ring + b * Kt::BUF;
         fq.issue((const T*)p.q + row * p.q_tok + (int64_t)head * p.q_head, left, buf);
         fo.issue((const T*)p.go + (row * p.heads_q + head) * p.dim, left, buf + Tl::BYTES);
-        // 64 floats each: statistics of rows behind the tile are fetched, too, and not used; those behind the sequence become
-        // 0 (their Q and dO are zeros)
+        // 64 floats each (by every wave of the group, the same values): those behind the tile are not used, those behind the
+        // sequence become 0 (their Q and dO are zeros)
         const int64_t at = (int64_t)head * p.total_q + row;
         const int bytes = (left < 64 ? left : 64) * 4;
 #pragma unroll
         for (int u = 0; u <= Stats<T>::N; ++u) {
             const float* src = (u == 0 ? p.delta : p.stats + (u - 1) * (int64_t)p.heads_q * p.total_q) + at;
-            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), 0, bytes, 0x00020000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LDS_PTR void*)(buf + 2 * Tl::BYTES + u * 256), 4, lane * 4, 0, 0, 0);
+            dma4(buffer_desc(src, bytes), lane * 4, buf + 2 * Tl::BYTES + u * 256);
         }
     };
+    constexpr int LOADS = 2 * Filler<T, DPAD, 32, SHARE>::N + 1 + Stats<T>::N;
     const int rbase = Tl::row_base(lane), cbase = Tl::col_base(lane);
-    Step cur = {0, wave - WAVES}, next = cur;
-    if (ntiles > 0) {
-        next = cur = advance(cur);
+    // Steps of this group; waves that share barriers take as many rounds as the first group, on zeros at the end.  Nothing is
+    // skipped inside the loop (keys behind the sequence, tiles above the diagonal): with a way around the products the compiler
+    // copies the sums at every turn, 15 % of the time for heads of 128.
+    const int rounds = (ntiles * p.group + GROUPS - 1 - (SHARE > 1 ? 0 : group)) / GROUPS;
+    Step cur = {0, 0}, next = cur;
+    if (rounds > 0) {
+        next = cur = advance(cur, group);
 #pragma unroll
-        for (int u = 0; u < Kt::STAGES - 1; ++u) { fill(next, u); next = advance(next); }
+        for (int u = 0; u < STAGES - 1; ++u) { fill(next, u); next = advance(next, GROUPS); }
     }
     int b = 0;
-    for (; ntiles > 0 && cur.g < p.group; cur = advance(cur), b = b + 1 == Kt::STAGES ? 0 : b + 1) {
-        wait_lds();                                   // the buffer filled next was read in the step before
-        fill(next, b == 0 ? Kt::STAGES - 1 : b - 1);
-        next = advance(next);
-        wait_loads<(Kt::STAGES - 1) * Kt::LOADS>();
+    for (int round = 0; round < rounds; ++round, cur = advance(cur, GROUPS), b = b + 1 == STAGES ? 0 : b + 1) {
+        wait_loads<(STAGES - 2) * LOADS>();
+        if constexpr (SHARE > 1) barrier();           // this round's tiles are complete, nobody reads the last round's any more
+        else wait_lds();
+        fill(next, b == 0 ? STAGES - 1 : b - 1);
+        next = advance(next, GROUPS);
         const int qb = (first + ntiles - 1 - cur.t) * 32;
         const char *qt = ring + b * Kt::BUF, *ot = qt + Tl::BYTES;
         const float *delta = reinterpret_cast<const float*>(ot + Tl::BYTES), *ref = delta + 64, *inv = ref + 64;
-        f32x16 sc[KB], dp[KB];
-#pragma unroll
-        for (int n = 0; n < KB; ++n) sc[n] = dp[n] = f32x16{};
-#pragma unroll
-        for (int d = 0; d < DPAD / 16; ++d) {
-            const Frag f = Tl::row(qt, rbase, 0, d);
-#pragma unroll
-            for (int n = 0; n < KB; ++n) sc[n] = Elem<T>::mma(f, kf[n][d], sc[n]);
-        }
-#pragma unroll
-        for (int d = 0; d < DPAD / 16; ++d) {
-            const Frag f = Tl::row(ot, rbase, 0, d);
-#pragma unroll
-            for (int n = 0; n < KB; ++n) dp[n] = Elem<T>::mma(f, vf[n][d], dp[n]);
-        }
-        const bool edge = p.causal && row0 + KEYS - 1 > qb + shift;
+        f32x16 sc = f32x16{}, dp = f32x16{};
+        pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::row(i < DPAD / 16 ? qt : ot, rbase, 0, i % (DPAD / 16)); }, [&](int i, Frag f) {
+            if (i < DPAD / 16) sc = Elem<T>::mma(f, kf[i], sc);
+            else dp = Elem<T>::mma(f, vf[i - DPAD / 16], dp);
+        });
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const f4 rf = *reinterpret_cast<const f4*>(ref + r * 8 + half * 4), de = *reinterpret_cast<const f4*>(delta + r * 8 + half * 4);
             f4 iv;
             if constexpr (Stats<T>::N == 2) iv = *reinterpret_cast<const f4*>(inv + r * 8 + half * 4);
 #pragma unroll
-            for (int n = 0; n < KB; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float pr = score_exp<T>(sc[n][r * 4 + i], p.scale_log2, rf[i]);
-                    if constexpr (Stats<T>::N == 2) pr *= iv[i];
-                    sc[n][r * 4 + i] = pr;
-                    dp[n][r * 4 + i] = pr * (dp[n][r * 4 + i] - de[i]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                float pr = score_exp<T>(sc[r * 4 + i], p.scale_log2, rf[i]);
+                if constexpr (Stats<T>::N == 2) pr *= iv[i];
+                sc[r * 4 + i] = pr;
+                dp[r * 4 + i] = pr * (dp[r * 4 + i] - de[i]);
+            }
         }
-        if (edge) {
+        if (p.causal && kw0 + 31 > qb + shift) {
 #pragma unroll
-            for (int n = 0; n < KB; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (row0 + n * 32 + (lane & 31) > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[n][i] = dp[n][i] = 0.f;
+            for (int i = 0; i < 16; ++i)
+                if (ki > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[i] = dp[i] = 0.f;
         }
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int c = 0; c < DPAD / 32; ++c) {
-                    const Frag fo_ = Tl::col(ot, cbase, c, k), fq_ = Tl::col(qt, cbase, c, k);
-#pragma unroll
-                    for (int n = 0; n < KB; ++n) {
-                        dv[n][c] = Elem<T>::mma(fo_, frag_of<T>(sc[n], k), dv[n][c]);
-                        dk[n][c] = Elem<T>::mma(fq_, frag_of<T>(dp[n], k), dk[n][c]);
-                    }
-                }
-        } else {
-            Frag x[2][DPAD / 32];
-            Tl::template cols<0>(x, ot, cbase);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int n = 0; n < KB; ++n) {
-                    const Frag pf = frag_of<T>(sc[n], k);
-#pragma unroll
-                    for (int c = 0; c < DPAD / 32; ++c) dv[n][c] = Elem<T>::mma(x[k][c], pf, dv[n][c]);
-                }
-            Tl::template cols<0>(x, qt, cbase);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int n = 0; n < KB; ++n) {
-                    const Frag df = frag_of<T>(dp[n], k);
-#pragma unroll
-                    for (int c = 0; c < DPAD / 32; ++c) dk[n][c] = Elem<T>::mma(x[k][c], df, dk[n][c]);
-                }
-        }
+        Frag pf, df;
+        pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::col(i % 2 ? qt : ot, cbase, i / 2 % (DPAD / 32), i / 2 / (DPAD / 32)); },
+                                            [&](int i, Frag f) {
+            const int c = i / 2 % (DPAD / 32), k = i / 2 / (DPAD / 32);
+            if (c == 0 && i % 2 == 0) { pf = frag_of<T>(sc, k); df = frag_of<T>(dp, k); }
+            if (i % 2) dk[c] = Elem<T>::mma(f, df, dk[c]);
+            else dv[c] = Elem<T>::mma(f, pf, dv[c]);
+        });
     }
 
-    // join: [wave][key][dim] fp32 in LDS, dV first, then dK
+    // join: [group][key][dim] fp32 in LDS, dV first, then dK
     wait_loads<0>();
     float* joined = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         barrier();                                    // the rings are done with, or the sums of dV have been read
 #pragma unroll
-        for (int n = 0; n < KB; ++n)
+        for (int c = 0; c < DPAD / 32; ++c)
 #pragma unroll
-            for (int c = 0; c < DPAD / 32; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x16& a = which ? dk[n][c] : dv[n][c];
-                    *reinterpret_cast<f4*>(joined + (wave * KEYS + n * 32 + (lane & 31)) * Kt::PAD + c * 32 + r * 8 + half * 4) =
-                        f4{a[r * 4], a[r * 4 + 1], a[r * 4 + 2], a[r * 4 + 3]};
-                }
+            for (int r = 0; r < 4; ++r) {
+                const f32x16& a = which ? dk[c] : dv[c];
+                *reinterpret_cast<f4*>(joined + (wave * 32 + (lane & 31)) * Kt::PAD + c * 32 + r * 8 + half * 4) =
+                    f4{a[r * 4], a[r * 4 + 1], a[r * 4 + 2], a[r * 4 + 3]};
+            }
         __syncthreads();
         const float f = which ? p.scale : 1.f;
-        for (int e = threadIdx.x; e < KEYS * (DPAD / 4); e += 64 * WAVES) {
-            const int key = e / (DPAD / 4), d = e % (DPAD / 4) * 4, ki = row0 + key;
-            if (ki >= sq.kcap || d >= p.dim) continue;
+        for (int e = threadIdx.x; e < KEYS * (DPAD / 4); e += 256) {
+            const int key = e / (DPAD / 4), d = e % (DPAD / 4) * 4, row = row0 + key;
+            if (row >= sq.kcap || d >= p.dim) continue;
             f4 v = {0.f, 0.f, 0.f, 0.f};
-            if (ki < sq.lk)                           // rows of the slot behind its keys get zeros
+            if (row < sq.lk)                          // rows of the slot behind its keys get zeros
 #pragma unroll
-                for (int u = 0; u < WAVES; ++u) v += *reinterpret_cast<const f4*>(joined + (u * KEYS + key) * Kt::PAD + d);
-            store4((T*)(which ? p.dk : p.dv) + ((int64_t)(sq.k0 + ki) * p.heads_k + w.kvh) * p.dim + d, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+                for (int g = 0; g < GROUPS; ++g) v += *reinterpret_cast<const f4*>(joined + (g * KEYS + key) * Kt::PAD + d);
+            store4((T*)(which ? p.dk : p.dv) + ((int64_t)(sq.k0 + row) * p.heads_k + w.kvh) * p.dim + d, v[0] * f, v[1] * f, v[2] * f, v[3] * f);
         }
     }
 }
 
 // delta and dQ: as the forward, with dO beside Q in registers and K read by columns, too.
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attention_dq_kernel(Params p)
+__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIMD((sizeof(T) * DPAD <= 256 ? 2 : 1)) void attention_dq_kernel(Params p)
 {
     typedef Tile<T, DPAD, BN> Tl;
     typedef typename Elem<T>::Frag Frag;
@@ -247,6 +210,9 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
         if (present && half == 0) p.delta[stat] = delta;
     }
 
+    settle(qf);
+    settle(of);
+    asm volatile("" ::"v"(ref), "v"(delta));
     const int see = p.causal ? min(sq.lk, qi + 1 + shift) : sq.lk;
     const int see_first = p.causal ? min(sq.lk, row0 + wave * 32 + 1 + shift) : sq.lk;
     const int see_wave = p.causal ? min(sq.lk, row0 + wave * 32 + 32 + shift) : sq.lk;
@@ -273,21 +239,27 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
         for (int u = 0; u < STAGES - 1; ++u) fill(u, u);
     }
     int b = 0;
-    for (int t = 0; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+    auto turn = [&](int t) {
         wait_loads<(STAGES - 2) * 2 * Filler<T, DPAD, BN, 4>::N>();
         barrier();                                   // tile t is complete, nobody reads the buffer of tile t - 1 any more
         fill(t + STAGES - 1, b == 0 ? STAGES - 1 : b - 1);
+    };
+    // Tiles above the diagonal for all of this wave's queries come last and only need its part of the ring.  (A branch around
+    // the products would make the compiler copy the sums at every turn.)
+    const int mine = min(tiles, (max(see_wave, 0) + BN - 1) / BN);
+    int t = 0;
+    for (; t < mine; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+        turn(t);
         const int key0 = t * BN;
-        if (key0 >= see_wave) continue;
         const char *kt = lds + b * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
         const bool edge = key0 + BN > see_first;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f32x16 sc = f32x16{}, dp = f32x16{};
-#pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) sc = Elem<T>::mma(Tl::row(kt, rbase, n, d), qf[d], sc);
-#pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) dp = Elem<T>::mma(Tl::row(vt, rbase, n, d), of[d], dp);
+            pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::row(i % 2 ? vt : kt, rbase, n, i / 2); }, [&](int i, Frag f) {
+                if (i % 2) dp = Elem<T>::mma(f, of[i / 2], dp);
+                else sc = Elem<T>::mma(f, qf[i / 2], sc);
+            });
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 dp[i] = score_exp<T>(sc[i], p.scale_log2, ref) * (dp[i] - delta);
@@ -306,17 +278,16 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
                     acc[c] += part;
                 }
             } else {
-                Frag x[2][DPAD / 32];
-                n == 0 ? Tl::template cols<0>(x, kt, cbase) : Tl::template cols<2>(x, kt, cbase);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const Frag df = frag_of<T>(dp, k);
-#pragma unroll
-                    for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(x[k][c], df, acc[c]);
-                }
+                Frag df;
+                pipelined<Frag, DPAD / 16, BATCH<T>>([&](int i) { return Tl::col(kt, cbase, i % (DPAD / 32), n * 2 + i / (DPAD / 32)); }, [&](int i, Frag f) {
+                    const int c = i % (DPAD / 32);
+                    if (c == 0) df = frag_of<T>(dp, i / (DPAD / 32));
+                    acc[c] = Elem<T>::mma(f, df, acc[c]);
+                });
             }
         }
     }
+    for (; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) turn(t);
     wait_loads<0>();
     if (!present) return;
     float f = p.scale;
@@ -352,7 +323,7 @@ static int launch_bwd_d(const Params& p, hipStream_t st) {
     }
     if (p.total_k > 0) {
         if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, Kt::LDS)) return rc;
-        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 64 * Kt::WAVES, Kt::LDS, st>>>(p);
+        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 256, Kt::LDS, st>>>(p);
         SEMPYR_CHECK_LAUNCH();
     }
     return 0;

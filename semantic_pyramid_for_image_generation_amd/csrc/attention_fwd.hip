@@ -10,8 +10,11 @@
 namespace attn {
 
 
+// waves a SIMD holds, by registers
+template <typename T, int DPAD> constexpr int fwd_waves() { return sizeof(T) * DPAD <= 128 ? 3 : sizeof(T) * DPAD <= 256 ? 2 : 1; }
+
 template <typename T, int DPAD>
-__global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attention_fwd_kernel(Params p)
+__global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_waves<T, DPAD>())) void attention_fwd_kernel(Params p)
 {
     typedef Tile<T, DPAD, BN> Tl;
     typedef typename Elem<T>::Frag Frag;
@@ -29,6 +32,8 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
 
     Frag qf[DPAD / 16];
     load_row_frags<T, DPAD>(qf, (const T*)p.q + (int64_t)(sq.q0 + qi) * p.q_tok + (int64_t)head * p.q_head, present, p.dim, lane);
+
+    settle(qf);
 
     // keys this lane's query sees, those the wave's first and the workgroup's last query see
     const int see = p.causal ? min(sq.lk, qi + 1 + shift) : sq.lk;
@@ -59,18 +64,22 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
         for (int u = 0; u < STAGES - 1; ++u) fill(u, u);
     }
     int b = 0;
-    for (int t = 0; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+    auto turn = [&](int t) {
         wait_loads<(STAGES - 2) * 2 * Filler<T, DPAD, BN, 4>::N>();
         barrier();                                   // tile t is complete, nobody reads the buffer of tile t - 1 any more
         fill(t + STAGES - 1, b == 0 ? STAGES - 1 : b - 1);
+    };
+    // Tiles above the diagonal for all of this wave's queries come last and only need its part of the ring.  (A branch around
+    // the products would make the compiler copy the sums at every turn.)
+    const int mine = min(tiles, (max(see_wave, 0) + BN - 1) / BN);
+    int t = 0;
+    for (; t < mine; ++t, b = b + 1 == STAGES ? 0 : b + 1) {
+        turn(t);
         const int key0 = t * BN;
-        if (key0 >= see_wave) continue;              // above the diagonal for all of this wave's queries
         const char *kt = lds + b * 2 * Tl::BYTES, *vt = kt + Tl::BYTES;
         f32x16 sc[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int d = 0; d < DPAD / 16; ++d) sc[b] = Elem<T>::mma(Tl::row(kt, rbase, b, d), qf[d], sc[b]);
+        pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::row(kt, rbase, i % 2, i / 2); },
+                                         [&](int i, Frag f) { sc[i % 2] = Elem<T>::mma(f, qf[i / 2], sc[i % 2]); });
         if (key0 + BN > see_first) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -115,21 +124,15 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) void attentio
                 for (int i = 0; i < 16; ++i) acc[b][i] += part[i];
             }
         } else {
-            Frag vf[2][DPAD / 32];
-            auto products = [&](const f32x16& x) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const Frag pf = frag_of<T>(x, k);
-#pragma unroll
-                    for (int b = 0; b < DPAD / 32; ++b) acc[b] = Elem<T>::mma(vf[k][b], pf, acc[b]);
-                }
-            };
-            Tl::template cols<0>(vf, vt, cbase);
-            products(sc[0]);
-            Tl::template cols<2>(vf, vt, cbase);
-            products(sc[1]);
+Frag pf;
+            pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::col(vt, cbase, i % (DPAD / 32), i / (DPAD / 32)); }, [&](int i, Frag f) {
+                const int k = i / (DPAD / 32), b = i % (DPAD / 32);
+                if (b == 0) pf = frag_of<T>(sc[k / 2], k % 2);
+                acc[b] = Elem<T>::mma(f, pf, acc[b]);
+            });
         }
     }
+    for (; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) turn(t);
     wait_loads<0>();
     l = half_sum(l);                                 // each lane half has summed its own keys
     if (!present) return;

@@ -56,6 +56,8 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
     load_row_frags<T, DPAD>(qf, (const T*)p.q + (int64_t)(sq.q0 + qi) * p.q_tok + (int64_t)(kvh * p.group + head_of(col)) * p.q_head,
                             present, p.dim, lane);
 
+    settle(qf);
+
     const int last = min(row0 + QT, sq.lq);          // queries of the tile end here
     const int see = p.causal ? min(sq.lk, qi + 1 + shift) : sq.lk;
     const int see_first = p.causal ? min(sq.lk, row0 + 1 + shift) : sq.lk;
@@ -122,22 +124,11 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
             sum += sc[i];
         }
         l += sum;
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag pf = frag_of<T>(sc, k);
+        for (int k = 0; k < 2; ++k) {
+            const Frag pf = frag_of<T>(sc, k);
 #pragma unroll
-                for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(vt, cbase, c, k), pf, acc[c]);
-            }
-        } else {
-            Frag vf[2][DPAD / 32];
-            Tl::template cols<0>(vf, vt, cbase);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag pf = frag_of<T>(sc, k);
-#pragma unroll
-                for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(vf[k][c], pf, acc[c]);
-            }
+            for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(vt, cbase, c, k), pf, acc[c]);
         }
     }
     l = half_sum(l);

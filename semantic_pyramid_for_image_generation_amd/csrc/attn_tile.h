@@ -22,6 +22,8 @@ namespace attn {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 #define LDS_PTR __attribute__((address_space(3)))
+// Tells the scheduler how many waves a SIMD will hold, so that it spends the registers on loads ahead of their use.
+#define WAVES_PER_SIMD(n) __attribute__((amdgpu_waves_per_eu(n, n)))
 
 struct Params {
     const void *q, *k, *v;                                   // [rows][heads][dim], strides in elements
@@ -101,56 +103,51 @@ struct Tile {
         }
         return h * 4 * ROWB + (((lane & 31) >> 2 ^ swz(h * 4)) << 4) + (lane & 3) * 4;
     }
-    // fp32: column 32 block + lane % 32, rows 16 t + 8 (j / 4) + 4 h + j % 4
+    // column 32 block + lane % 32, rows 16 t + 8 (j / 4) + 4 h + j % 4
     static __device__ __forceinline__ Frag col(const char* tile, int base, int block, int t) {
-        static_assert(SZ == 4, "16-bit types read their columns with cols()");
-        Frag f;
+        if constexpr (SZ == 2) {
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            V4 x[2];                                         // (cast as a whole: __builtin_bit_cast of one element takes element 0)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = (j / 4) * 8 + j % 4;
-            f[j] = *reinterpret_cast<const float*>(tile + (t * 16 + r) * ROWB + (base ^ block * 128 ^ swz(r) << 4));
-        }
-        return f;
-    }
-    // 16-bit types: the same of groups T and T + 1 for all column blocks, f[group][block].  Written in assembly because the
-    // compiler puts a wait for ALL vector memory before the builtin of a transposing read, also for the DMA that fills other
-    // buffers; the reads' own wait is part of the block.
-    template <int T0>
-    static __device__ __forceinline__ void cols(Frag (&f)[2][DPAD / 32], const char* tile, int base) {
-        static_assert(SZ == 2, "fp32 reads its columns with col()");
-        constexpr int O = T0 * 16 * ROWB, G = 16 * ROWB, H = 8 * ROWB;      // first group; next group; second half of a group
-        const unsigned at = (unsigned)(uintptr_t)(LDS_PTR const char*)tile;
-        typedef T V4 __attribute__((ext_vector_type(4)));
-        if constexpr (DPAD == 32) {
-            s16x4 x[4];
-            asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %5 offset:%7\n\t"
-                         "ds_read_b64_tr_b16 %2, %4 offset:%8\n\tds_read_b64_tr_b16 %3, %5 offset:%9\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
-                         : "v"(at + base), "v"(at + (base ^ 32)), "n"(O), "n"(O + H), "n"(O + G), "n"(O + G + H) : "memory");
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-                f[g][0] = __builtin_shufflevector(__builtin_bit_cast(V4, x[2 * g]), __builtin_bit_cast(V4, x[2 * g + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+            for (int u = 0; u < 2; ++u)
+                x[u] = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LDS_PTR s16x4*)(tile + (t * 16 + u * 8) * ROWB + (base ^ block * 64 ^ u * 32))));
+            return __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
+            Frag f;
 #pragma unroll
-            for (int c = 0; c < DPAD / 32; c += 2) {
-                s16x4 x[8];                               // [group][block][half]
-                asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%13\n\t"
-                             "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%13\n\t"
-                             "ds_read_b64_tr_b16 %4, %8 offset:%14\n\tds_read_b64_tr_b16 %5, %9 offset:%15\n\t"
-                             "ds_read_b64_tr_b16 %6, %10 offset:%14\n\tds_read_b64_tr_b16 %7, %11 offset:%15\n\ts_waitcnt lgkmcnt(0)"
-                             : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
-                             : "v"(at + (base ^ c * 64)), "v"(at + (base ^ c * 64 ^ 32)), "v"(at + (base ^ (c + 1) * 64)),
-                               "v"(at + (base ^ (c + 1) * 64 ^ 32)), "n"(O), "n"(O + H), "n"(O + G), "n"(O + G + H) : "memory");
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        f[g][c + u] = __builtin_shufflevector(__builtin_bit_cast(V4, x[g * 4 + u * 2]), __builtin_bit_cast(V4, x[g * 4 + u * 2 + 1]),
-                                                              0, 1, 2, 3, 4, 5, 6, 7);
+            for (int j = 0; j < 8; ++j) {
+                const int r = (j / 4) * 8 + j % 4;
+                f[j] = *reinterpret_cast<const float*>(tile + (t * 16 + r) * ROWB + (base ^ block * 128 ^ swz(r) << 4));
             }
+            return f;
         }
     }
 };
+
+// LDS DMA of 16 (4) bytes a lane: lane i's bytes from `offset` in the buffer go to lds + 16 i (4 i); behind the buffer's end zeros.
+// In assembly, because the compiler, where it knows of a DMA in flight, waits for all of them before a transposing LDS read,
+// whatever buffer that reads; the waits are wait_loads() here.  Nothing is returned in registers.
+typedef int BufferDesc __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ BufferDesc buffer_desc(const void* base, int bytes) {
+    const uint64_t at = (uint64_t)base;
+    return BufferDesc{__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xFFFF),
+                      __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
+}
+__device__ __forceinline__ unsigned lds_offset(const void* p) { return (unsigned)(uintptr_t)(LDS_PTR const char*)p; }
+// (m0, the DMA's LDS address, is a reserved register: the compiler warns that it does not keep a value there across the block,
+// which is what the clobber says)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(BufferDesc rsrc, int offset, const void* lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds_offset(lds))), "v"(offset), "s"(rsrc) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(BufferDesc rsrc, int offset, const void* lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds_offset(lds))), "v"(offset), "s"(rsrc) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 
 // Fills tiles from rows of a strided tensor.  `waves` waves share a tile; a lane's source offsets are fixed.
 template <typename T, int DPAD, int ROWS, int WAVES>
@@ -175,10 +172,9 @@ struct Filler {
     __device__ __forceinline__ void issue(const void* base, int valid, char* tile) const {
         const int rows = valid < ROWS ? valid : ROWS;
         const int bytes = rows > 0 ? (rows - 1) * stride_bytes + row_bytes : 0;
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+        const BufferDesc rsrc = buffer_desc(base, bytes);
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LDS_PTR void*)(tile + (j * WAVES + wave) * 1024), 16, voff[j], 0, 0, 0);
+        for (int j = 0; j < N; ++j) dma16(rsrc, voff[j], tile + (j * WAVES + wave) * 1024);
     }
 };
 
@@ -217,6 +213,38 @@ __device__ __forceinline__ float half_max(float x) {
 __device__ __forceinline__ float half_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// STEPS products from fragments read from LDS, in batches: the next batch is read before this one is used, and the scheduler
+// may move neither reads nor products across (left alone, the compiler reads every fragment into the same registers right
+// before its product, which then waits for the LDS each time).
+template <typename T> constexpr int BATCH = sizeof(T) == 4 ? 2 : 4;
+template <typename F, int STEPS, int MOST, typename Load, typename Use>
+__device__ __forceinline__ void pipelined(Load load, Use use) {
+    constexpr int BATCH = MOST < STEPS ? MOST : STEPS, N = STEPS / BATCH, VALU_SALU_MAY_CROSS = 0x6;
+    static_assert(STEPS % BATCH == 0, "whole batches");
+    F f[2][BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) f[0][i] = load(i);
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+        if (s + 1 < N) {
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) f[(s + 1) & 1][i] = load((s + 1) * BATCH + i);
+        }
+        __builtin_amdgcn_sched_barrier(VALU_SALU_MAY_CROSS);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) use(s * BATCH + i, f[s & 1][i]);
+        __builtin_amdgcn_sched_barrier(VALU_SALU_MAY_CROSS);
+    }
+}
+
+// Settles loads into registers before a loop: the compiler would otherwise place their wait inside it, where it would also wait
+// for the DMA in flight.
+template <typename F, int N>
+__device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 
 // 4 consecutive elements
