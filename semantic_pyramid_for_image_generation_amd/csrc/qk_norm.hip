@@ -244,23 +244,26 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeParams q)
     }
 }
 
-// dw[part][d] = sum over blocks of partials[block][part][d]: 8 columns a workgroup, 32 threads a column, fixed order.
+// dw[part][d] = sum over blocks of partials[block][part][d]: 8 columns a workgroup, 128 threads a column, fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void weight_grad_kernel(const float* __restrict__ partials, int blocks, int dim, T* __restrict__ dwq,
-                                                          T* __restrict__ dwk)
+__global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restrict__ partials, int blocks, int dim, T* __restrict__ dwq,
+                                                           T* __restrict__ dwk)
 {
-    const int col = blockIdx.x * 8 + threadIdx.x % 8, row0 = threadIdx.x / 8;
+    const int c = threadIdx.x % 8, col = blockIdx.x * 8 + c, row0 = threadIdx.x / 8;
     float t = 0.f;
-    if (col < 2 * dim)
-        for (int r = row0; r < blocks; r += 32) t += partials[(int64_t)r * 2 * dim + col];
-    __shared__ float sh[32][9];
-    sh[row0][threadIdx.x % 8] = t;
-    __syncthreads();
-    if (threadIdx.x < 8 && col < 2 * dim) {
-        float u = 0.f;
-        for (int r = 0; r < 32; ++r) u += sh[r][threadIdx.x];
-        (col < dim ? dwq : dwk)[col < dim ? col : col - dim] = (T)u;
+    if (col < 2 * dim) {
+#pragma unroll 8
+        for (int r = row0; r < blocks; r += 128) t += partials[(int64_t)r * 2 * dim + col];
     }
+    __shared__ float sh[128][9];
+    sh[row0][c] = t;
+    __syncthreads();
+#pragma unroll
+    for (int half = 64; half > 0; half /= 2) {
+        if (row0 < half) sh[row0][c] += sh[row0 + half][c];
+        __syncthreads();
+    }
+    if (row0 == 0 && col < 2 * dim) (col < dim ? dwq : dwk)[col < dim ? col : col - dim] = (T)sh[0][c];
 }
 
 constexpr int MAX_BLOCKS = 1024;                       // backward: four workgroups a CU, one row of partial sums each
@@ -387,7 +390,7 @@ extern "C" int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq
             if (int rc = launch<T, true>(q, l, (unsigned)blocks, st)) return rc;
         }
         if (!wq) return 0;
-        weight_grad_kernel<T><<<ceil_div(2 * d->dim, 8), 256, 0, st>>>(scratch, (int)blocks, d->dim, (T*)dwq, (T*)dwk);
+        weight_grad_kernel<T><<<ceil_div(2 * d->dim, 8), 1024, 0, st>>>(scratch, (int)blocks, d->dim, (T*)dwq, (T*)dwk);
         SEMPYR_CHECK_LAUNCH();
         return 0;
     });

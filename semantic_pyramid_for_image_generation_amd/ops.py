@@ -8,6 +8,7 @@ discriminator uses.  There is no CPU path: non-CUDA(HIP) tensors raise.
 """
 import ctypes
 import fractions
+import functools
 import os
 import threading
 
@@ -1827,28 +1828,24 @@ def lerp_rows(real, fake, alpha):
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _token_dtype(tensors, what):
-    """The common element-type code of `tensors` (name -> tensor, None entries skipped)."""
-    dtypes = {t.dtype for t in tensors.values() if t is not None}
-    if len(dtypes) != 1 or next(iter(dtypes)) not in _DTYPE_CODE:
-        raise _lib.SempyrError(f"{what}: one type of float32, float16 or bfloat16 for all of {', '.join(tensors)} expected, got "
-                               + ", ".join(f"{n} {t.dtype}" for n, t in tensors.items() if t is not None))
-    return _DTYPE_CODE[next(iter(dtypes))]
-
-
-def _one_device(tensors, what):
-    """Refuses CPU tensors and tensors of several GPUs; returns the device."""
-    dev = None
-    for name, t in tensors.items():
+def _token_args(what, names, tensors, others=()):
+    """Checks what a token operator is called with: one floating type for `tensors` (None entries skipped), everything (also
+    `others`: index tensors) on one GPU.  Returns the element-type code."""
+    first = tensors[0]
+    code = _DTYPE_CODE.get(first.dtype)
+    if code is None or any(t is not None and t.dtype != first.dtype for t in tensors):
+        raise _lib.SempyrError(f"{what}: one type of float32, float16 or bfloat16 for all of {', '.join(names)} expected, got "
+                               + ", ".join(f"{n} {t.dtype}" for n, t in zip(names, tensors) if t is not None))
+    dev = first.device
+    for t in (*tensors, *others):
         if t is None:
             continue
         if not t.is_cuda:
-            raise _lib.SempyrError(f"{what}: {name}: the sempyr operators run on the GPU only (got a {t.device} tensor); "
-                                   "there is no CPU fallback")
-        if dev is not None and t.device != dev:
+            raise _lib.SempyrError(f"{what}: the sempyr operators run on the GPU only (got a {t.device} tensor); there is no CPU "
+                                   "fallback")
+        if t.device != dev:
             raise _lib.SempyrError(f"{what}: tensors on {dev} and {t.device}")
-        dev = t.device
-    return dev
+    return code
 
 
 class _on_device:
@@ -1895,6 +1892,7 @@ class AxialRope:
         self.base, self.interleaved, self.shared = float(base), bool(interleaved), bool(shared)
         self.pairs = sum(self.sections)
         self._tables = {}
+        self._sections_c = (ctypes.c_int32 * 4)(*self.sections)
 
     def frequencies(self):
         """The angle of one position step, per pair (radians)."""
@@ -1919,9 +1917,17 @@ class AxialRope:
 
 
 def _rope_desc(q, k, rope, dtype, eps):
-    sec = list(rope.sections) + [0] * (4 - len(rope.sections))
-    return _lib.RopeDesc(q.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), dtype, q.shape[1], k.shape[1], q.shape[2],
-                         len(rope.sections), (ctypes.c_int32 * 4)(*sec), int(rope.interleaved), eps)
+    (tokens, heads_q, dim), (qt, qh, _), (kt, kh, _) = q.shape, q.stride(), k.stride()
+    return _lib.RopeDesc(tokens, qt, qh, kt, kh, dtype, heads_q, k.shape[1], dim, len(rope.sections), rope._sections_c,
+                         rope.interleaved, eps)
+
+
+@functools.lru_cache(maxsize=None)
+def _rope_scratch(dim):
+    n = ctypes.c_int64()
+    desc = _lib.RopeDesc(0, 0, 0, 0, 0, _lib.F32, 1, 1, dim, 1, (ctypes.c_int32 * 4)(1), 0, 0.0)
+    check(L.sempyr_qk_norm_rope_bwd_scratch(ctypes.byref(desc), ctypes.byref(n)), "sempyr_qk_norm_rope_bwd_scratch")
+    return n.value
 
 
 class _QkNormRope(Function):
@@ -1931,31 +1937,27 @@ class _QkNormRope(Function):
             q, k, positions = _rows(q), _rows(k), positions.contiguous()
             if wq is not None:
                 wq, wk = wq.contiguous(), wk.contiguous()
-            yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            check(L.sempyr_qk_norm_rope_fwd(ctypes.byref(_rope_desc(q, k, rope, dtype, eps)), q.data_ptr(), k.data_ptr(),
-                                            positions.data_ptr(), rope.table(q.device).data_ptr(), _p(wq), _p(wk), yq.data_ptr(),
-                                            yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
+            yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
+            desc = ctypes.byref(_rope_desc(q, k, rope, dtype, eps))
+            check(L.sempyr_qk_norm_rope_fwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(), rope.table(q.device).data_ptr(),
+                                            _p(wq), _p(wk), yq.data_ptr(), yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
         ctx.save_for_backward(q, k, positions, wq, wk)
-        ctx.cfg = (rope, eps, dtype)
+        ctx.cfg = (rope, desc)
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
         _no_second_order("qk_norm_rope", gq, gk)
         q, k, positions, wq, wk = ctx.saved_tensors
-        rope, eps, dtype = ctx.cfg
+        rope, desc = ctx.cfg
         with _on_device(q.device):
             gq, gk = gq.contiguous(), gk.contiguous()
             dq, dk = torch.empty_like(gq), torch.empty_like(gk)
             dwq = dwk = scratch = None
-            desc = _rope_desc(q, k, rope, dtype, eps)
             if wq is not None:
-                n = ctypes.c_int64()
-                check(L.sempyr_qk_norm_rope_bwd_scratch(ctypes.byref(desc), ctypes.byref(n)), "sempyr_qk_norm_rope_bwd_scratch")
-                scratch = torch.empty(n.value, dtype=torch.float32, device=q.device)
+                scratch = torch.empty(_rope_scratch(q.shape[2]), dtype=torch.float32, device=q.device)
                 dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-            check(L.sempyr_qk_norm_rope_bwd(ctypes.byref(desc), q.data_ptr(), k.data_ptr(), positions.data_ptr(),
+            check(L.sempyr_qk_norm_rope_bwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(),
                                             rope.table(q.device).data_ptr(), _p(wq), _p(wk), gq.data_ptr(), gk.data_ptr(),
                                             dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), _p(scratch), _stream()),
                   "sempyr_qk_norm_rope_bwd")
@@ -1992,8 +1994,7 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps=1e-6):
             raise _lib.SempyrError(f"qk_norm_rope: weights of shape ({dim},) expected, got {tuple(w.shape)}")
     if not 0.0 <= eps < float("inf"):
         raise _lib.SempyrError(f"qk_norm_rope: eps must be finite and not negative, got {eps}")
-    dtype = _token_dtype({"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
-    _one_device({"q": q, "k": k, "positions": positions, "q_weight": q_weight, "k_weight": k_weight}, "qk_norm_rope")
+    dtype = _token_args("qk_norm_rope", ("q", "k", "q_weight", "k_weight"), (q, k, q_weight, k_weight), (positions,))
     return _apply(_QkNormRope, q, k, positions, rope, q_weight, k_weight, float(eps), dtype)
 
 
@@ -2009,8 +2010,16 @@ def _attn_rows(t):
 
 
 def _attn_desc(q, k, v, nseq, causal, scale, dtype):
-    return _lib.AttentionDesc(q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                              dtype, q.shape[1], k.shape[1], q.shape[2], nseq, causal, scale)
+    (total_q, heads_q, dim), (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.shape, q.stride(), k.stride(), v.stride()
+    return _lib.AttentionDesc(total_q, k.shape[0], qt, qh, kt, kh, vt, vh, dtype, heads_q, k.shape[1], dim, nseq, causal, scale)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_workspace(total_q, total_k, heads_q, heads_k, dim, nseq, dtype):
+    n, row = ctypes.c_int64(), max(heads_q, heads_k) * dim
+    desc = _lib.AttentionDesc(total_q, total_k, row, dim, row, dim, row, dim, dtype, heads_q, heads_k, dim, nseq, 0, 1.0)
+    check(L.sempyr_attention_workspace(ctypes.byref(desc), ctypes.byref(n)), "sempyr_attention_workspace")
+    return n.value
 
 
 class _Attention(Function):
@@ -2020,34 +2029,31 @@ class _Attention(Function):
             q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
             len_k = len_k if len_k is None else len_k.contiguous()
-            o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            o = q.new_empty(q.shape)
             stats = low = None
             if any(ctx.needs_input_grad[:3]):
                 stats = torch.empty((2 if dtype == _lib.F32 else 1, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
                 low = torch.empty_like(o) if dtype != _lib.F32 else None
             desc = ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype))
-            n = ctypes.c_int64()
-            check(L.sempyr_attention_workspace(desc, ctypes.byref(n)), "sempyr_attention_workspace")
-            ws = _workspace(4 * n.value, q.device)
+            n = _attn_workspace(q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], cu_q.numel() - 1, dtype)
+            ws = _workspace(4 * n, q.device)
             check(L.sempyr_attention_fwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k),
-                                         o.data_ptr(), _p(low), _p(stats), _p(ws), n.value, _stream()), "sempyr_attention_fwd")
+                                         o.data_ptr(), _p(low), _p(stats), _p(ws), n, _stream()), "sempyr_attention_fwd")
         if stats is not None:
             ctx.save_for_backward(q, k, v, o, low, stats, cu_q, cu_k, len_k)
-            ctx.cfg = (causal, scale, dtype)
+            ctx.cfg = desc
         return o
 
     @staticmethod
     def backward(ctx, g):
         _no_second_order("attention", g)
         q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
-        causal, scale, dtype = ctx.cfg
         with _on_device(q.device):
             g = g.contiguous()
             g = g if g.data_ptr() % 16 == 0 else g.clone()
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             delta = torch.empty_like(stats[0])
-            check(L.sempyr_attention_bwd(ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype)), q.data_ptr(),
-                                         k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
+            check(L.sempyr_attention_bwd(ctx.cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
                                          cu_k.data_ptr(), _p(len_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                          delta.data_ptr(), _stream()), "sempyr_attention_bwd")
         return dq, dk, dv, None, None, None, None, None, None
@@ -2065,7 +2071,6 @@ def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
             q.shape[1] % k.shape[1]:
         raise _lib.SempyrError("attention: q [total_q, heads_q, dim] and k, v [total_k, heads_k, dim] with heads_q a multiple of "
                                f"heads_k expected, got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    dtype = _token_dtype({"q": q, "k": k, "v": v}, "attention")
     unit = 16 // q.element_size()
     if q.shape[2] % unit or q.shape[2] > 128:
         raise _lib.SempyrError(f"attention: a head dim that is a multiple of {unit}, at most 128, expected, got {q.shape[2]}")
@@ -2084,7 +2089,7 @@ def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
     scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise _lib.SempyrError(f"attention: scale must be positive and finite, got {scale}")
-    _one_device({"q": q, "k": k, "v": v, "cu_q": cu_q, "cu_k": cu_k, "len_k": len_k}, "attention")
+    dtype = _token_args("attention", ("q", "k", "v"), (q, k, v), (cu_q, cu_k, len_k))
     return _apply(_Attention, q, k, v, cu_q, cu_k, len_k, bool(causal), scale, dtype)
 
 
@@ -2092,7 +2097,7 @@ def _dropout_raw(x, res, p, rng, dtype):
     with _on_device(x.device):
         x = x.contiguous()
         res = res if res is None else res.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x)
         check(L.sempyr_dropout_add(dtype, x.data_ptr(), _p(res), y.data_ptr(), x.numel(), p, rng.data_ptr(), _stream()),
               "sempyr_dropout_add")
     return y
@@ -2126,6 +2131,5 @@ def dropout_add(x, res, p, rng):
         raise _lib.SempyrError(f"dropout_add: p must lie in [0, 1], got {p}")
     if rng.dtype != torch.int64 or rng.numel() != 2:
         raise _lib.SempyrError("dropout_add: rng must be an int64 tensor {seed, offset}")
-    dtype = _token_dtype({"x": x, "res": res}, "dropout_add")
-    _one_device({"x": x, "res": res, "rng": rng}, "dropout_add")
+    dtype = _token_args("dropout_add", ("x", "res"), (x, res), (rng,))
     return _apply(_DropoutAdd, x, res, p, rng, dtype)
