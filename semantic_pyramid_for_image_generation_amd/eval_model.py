@@ -49,7 +49,7 @@ def synthesize_batch(generator, classifier, images, normalizer_clf, num_levels=4
 def _main():
     from . import imageio
     device = parallel.init_device()
-    generator = Generator(gen_type=args.gen_type)
+    generator = Generator(gen_type=args.gen_type, attention_size=args.attention_size)
     generator.load_state_dict(torch.load(args.generator_path, map_location='cpu', weights_only=True))
     generator.eval()
     generator.to(device)
@@ -88,6 +88,7 @@ def build_parser():
     parser.add_argument('--num-of-noises', default=4, type=int)
     parser.add_argument('--output-path', required=True)
     parser.add_argument('--gen-type', default='res', choices=['default', 'res'])
+    parser.add_argument('--attention-size', default=0, type=int, choices=[0, 8, 16, 32, 64], help='self-attention over the generator maps of this size, 0 for none')
     parser.add_argument('--classifier-path', default='/home/dcor/ronmokady/workshop21/team1/try/classifier18')
     return parser
 

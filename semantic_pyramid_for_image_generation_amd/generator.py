@@ -8,6 +8,7 @@ import torch.nn as nn
 import os
 
 from . import ops
+from .attention import SelfAttention2d
 from .blocks import (init_weights, run_conv, run_conv_norm, run_conv_norm_act,  # noqa: F401  (init_weights re-exported)
                      run_norm, run_norm_add_norm_act, tail_takes_half_res, fuses_conv_norm, activation_kind, _single)
 
@@ -128,11 +129,17 @@ class GeneratorBlock(nn.Module):
 
 class Generator(nn.Module):
     """z (B,128,1,1) + masked classifier taps 1..4 -> image (B,3,256,256) in [-1,1]
-    (reference generator.py:97-145)."""
+    (reference generator.py:97-145).  `attention_size` S (8, 16, 32 or 64; 0: none, the reference's generator): a
+    SelfAttention2d behind the block that leaves SxS maps, its parameters under `attention` in the state_dict."""
 
-    def __init__(self, gen_type):
+    CHANNELS_AT = {8: 512, 16: 256, 32: 128, 64: 64}
+
+    def __init__(self, gen_type, attention_size=0, attention_dropout=0.0):
         super().__init__()
+        if attention_size and attention_size not in self.CHANNELS_AT:
+            raise ValueError(f"Generator: attention_size must be 0 or one of {sorted(self.CHANNELS_AT)}, got {attention_size}")
         self.gen_type = gen_type
+        self.attention_size = attention_size
         self.conv_block1 = ConvBlock(128, 512, 4, stride=1, padding=0)      # 1x1 -> 4x4
         self.conv_block2 = ConvBlock(512, 512, 4, stride=2, padding=1)      # 4x4 -> 8x8
         self.conv_block3 = GeneratorBlock(512, 256, gen_type)               # -> 16x16
@@ -145,12 +152,17 @@ class Generator(nn.Module):
             self.conv_block7 = ResidualBlock(64, 64)                        # -> 256x256
             self.last_conv = nn.Conv2d(64, 3, kernel_size=3, stride=1, padding=1)
         self.tanh = nn.Tanh()
+        if attention_size:              # constructed last: the other layers' seeded initial values stay what they are
+            self.attention = SelfAttention2d(self.CHANNELS_AT[attention_size], dropout=attention_dropout)
+
+    def _attend(self, x):
+        return self.attention(x) if self.attention_size and x.shape[2] == self.attention_size else x
 
     def forward(self, noise, features, masks):
         x = self.conv_block1(noise)
-        x = self.conv_block2(x)
+        x = self._attend(self.conv_block2(x))
         for level, block in ((4, self.conv_block3), (3, self.conv_block4), (2, self.conv_block5), (1, self.conv_block6)):
-            x = block(x, features[level], masks[level])
+            x = self._attend(block(x, features[level], masks[level]))
         if self.gen_type == 'res':
             x = self.conv_block7(x)
         return run_conv(self.last_conv, x, act_kind=ops.ACT_TANH)
@@ -160,6 +172,8 @@ class Generator(nn.Module):
                   self.conv_block6]
         if self.gen_type == 'res':
             blocks.append(self.conv_block7)
+        if self.attention_size:
+            blocks.append(self.attention)
         for blk in blocks:
             blk.init_weights()
         self.last_conv.apply(init_weights)

@@ -641,7 +641,7 @@ def _main():
     classifier.eval()
     for p in classifier.parameters():
         p.requires_grad_(False)
-    generator = Generator(gen_type=args.gen_type)
+    generator = Generator(gen_type=args.gen_type, attention_size=args.attention_size, attention_dropout=args.attention_dropout)
     discriminator = Discriminator(args.discriminator_norm, dis_type=args.gen_type)
     if args.generator_path is not None:
         generator.load_state_dict(torch.load(args.generator_path, map_location='cpu', weights_only=True))
@@ -801,6 +801,8 @@ def build_parser():
     parser.add_argument('--fixed-layer', type=int, help='train only this layer')
     parser.add_argument('--keep-temp-results', action='store_true')
     parser.add_argument('--use-diversity-loss', action='store_true')
+    parser.add_argument('--attention-size', default=0, type=int, choices=[0, 8, 16, 32, 64], help='self-attention over the generator maps of this size, 0 for none')
+    parser.add_argument('--attention-dropout', default=0.0, type=float)
     return parser
 
 

@@ -1,0 +1,221 @@
+"""The token operators together, as the generator's self-attention block uses them: against 64 bits, in the training loop, from
+captured graphs, on other streams."""
+import random
+from argparse import Namespace
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import token_oracle as oracle
+from oracle import recipes
+
+pytestmark = pytest.mark.gpu
+
+
+def block_in_64_bits(sd, x, heads, head_dim, gain=None):
+    """SelfAttention2d on the CPU in double; gain: the dropout's factors."""
+    B, C, H, W = x.shape
+    y = F.group_norm(x, 1, sd['norm.weight'], sd['norm.bias'], 1e-5)
+    y = F.conv2d(y, sd['qkv.weight'])
+    t = y.flatten(2).transpose(1, 2).reshape(B * H * W, 3, heads, head_dim)
+    i = torch.arange(B * H * W)
+    pos = torch.stack([i // W % H, i % W], dim=1)
+    rot = dict(positions=pos, sections=(head_dim // 4,) * 2, base=10000.0, interleaved=False, shared=False)
+    norm = lambda v, w: v * (v.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+    q, k = oracle.rotate(norm(t[:, 0], sd['q_weight']), **rot), oracle.rotate(norm(t[:, 1], sd['k_weight']), **rot)
+    per = lambda v: v.view(B, H * W, heads, head_dim).transpose(1, 2)
+    p = torch.softmax(per(q) @ per(k).transpose(2, 3) * head_dim ** -0.5, dim=-1)
+    o = (p @ per(t[:, 2])).transpose(1, 2).reshape(B, H * W, C).transpose(1, 2).reshape(B, C, H, W)
+    o = F.conv2d(o, sd['proj.weight'], sd['proj.bias'])
+    return x + (o if gain is None else o * gain.view(x.shape))
+
+
+# Ten fp32 stages in a row, each a sum of at most 1152 products: a stage adds at most 1152 u / 2 relative (its terms' errors do
+# not all agree), 3.5e-5 at worst and far less in the mean; relative L2 errors stay below ten of them.
+REL = 10 * 1152 * oracle.U / 2
+
+
+@pytest.mark.parametrize("shape", [(2, 128, 8, 8), (1, 64, 16, 12), (3, 32, 5, 7), (1, 256, 1, 1)])
+@pytest.mark.parametrize("dropout", [0.0, 0.25])
+def test_block(dev, shape, dropout):
+    from semantic_pyramid_for_image_generation_amd.attention import SelfAttention2d
+    torch.manual_seed(sum(shape))
+    blk = SelfAttention2d(shape[1], dropout=dropout)
+    for p in blk.parameters():
+        torch.nn.init.normal_(p, 1.0 if p.dim() == 1 else 0.0, 0.2 if p.dim() == 1 else shape[1] ** -0.5)
+    x, g = torch.randn(shape), torch.randn(shape)
+    sd = {k: v.detach().double().requires_grad_() for k, v in blk.state_dict().items()}
+    xd = x.double().requires_grad_()
+    seed, _ = blk.rng.tolist()
+    gain = oracle.dropout_gain(x.numel(), dropout, seed, 0) if dropout else None
+    want = block_in_64_bits(sd, xd, blk.heads, blk.head_dim, gain)
+    names = list(sd)
+    wants = torch.autograd.grad(want, [xd] + [sd[n] for n in names], g.double())
+    blk.to(dev).train()
+    xg = x.to(dev).requires_grad_()
+    got = blk(xg)
+    grads = torch.autograd.grad(got, [xg] + [blk.get_parameter(n) for n in names], g.to(dev))
+    assert blk.rng.tolist() == [seed, 1 if dropout else 0]
+    scale = max(float(w.norm()) for w in wants[1:])
+    for n, a, b in zip(['out', 'x'] + names, [got.detach(), *grads], [want.detach(), *wants]):
+        err = float((a.double().cpu() - b).norm())
+        # (a gradient that is zero by the mathematics -- the key weights of a map of one place -- is measured by the others)
+        assert err <= REL * max(float(b.norm()), 1e-3 * scale), (n, err, float(b.norm()))
+    blk.eval()
+    with torch.no_grad():
+        plain = block_in_64_bits({k: v.detach() for k, v in sd.items()}, x.double(), blk.heads, blk.head_dim)
+        assert float((blk(xg).double().cpu() - plain).norm()) <= REL * float(plain.norm())
+
+
+@pytest.mark.parametrize("gen_type,size", [('res', 32), ('default', 8)])
+def test_generator_runs_with_attention(dev, gen_type, size):
+    from semantic_pyramid_for_image_generation_amd.generator import Generator
+    torch.manual_seed(1)
+    g = Generator(gen_type, attention_size=size, attention_dropout=0.1); g.init_weights(); g.to(dev).train()
+    shapes = [None, (2, 64, 64, 64), (2, 128, 32, 32), (2, 256, 16, 16), (2, 512, 8, 8), None]
+    feats = [None if s is None else torch.randn(s, device=dev) for s in shapes]
+    masks = [None if f is None else torch.ones_like(f) for f in feats]
+    y = g(torch.randn(2, 128, 1, 1, device=dev), feats, masks)
+    y.square().mean().backward()
+    assert y.shape == (2, 3, 256, 256)
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in g.parameters())
+    assert float(g.attention.qkv.weight.grad.norm()) > 0
+    g.eval()
+    with torch.no_grad():
+        assert torch.isfinite(g(torch.randn(2, 128, 1, 1, device=dev), feats, masks)).all()
+
+
+@pytest.mark.parametrize("dropout", [0.0, 0.1])
+def test_training_loop_from_graphs(dev, dropout):
+    """The captured loop body with the block in the generator: the bits of eager execution, parameters and dropout's offset among
+    them."""
+    from semantic_pyramid_for_image_generation_amd import loop, optim
+    from semantic_pyramid_for_image_generation_amd import train_model as tm
+    from semantic_pyramid_for_image_generation_amd.classifier import Classifier, resnet18
+    from semantic_pyramid_for_image_generation_amd.discriminator import Discriminator
+    from semantic_pyramid_for_image_generation_amd.generator import Generator
+
+    def run(use_graphs):
+        torch.manual_seed(11)
+        G = Generator('res', attention_size=16, attention_dropout=dropout); G.init_weights()
+        D = Discriminator('instance_norm', 'res'); D.init_weights()
+        C = Classifier(resnet18(365)); C.load_state_dict(recipes.make_resnet(11).state_dict())
+        G.to(dev); D.to(dev); C.to(dev).eval()
+        for p in C.parameters():
+            p.requires_grad_(False)
+        tm.args = Namespace(use_diversity_loss=False, gradient_penalty_weight=10.0)
+        g_opt = optim.Adam(G.parameters(), lr=2e-4, betas=(0.5, 0.999), capturable=True)
+        d_opt = optim.Adam(D.parameters(), lr=2e-4, betas=(0.5, 0.999), capturable=True)
+        lp = loop.TrainLoop(G, D, C, g_opt, d_opt, 2, dev, use_graphs=use_graphs)
+        lp.prepare()
+        torch.manual_seed(7); random.seed(7)
+        for i in range(7):
+            lp.iteration(recipes.image_batch(40 + i % 3, 2).to(dev), log=True)
+        logged = lp.pop_logged()
+        torch.cuda.synchronize()
+        return logged, {**{('G', k): v.clone() for k, v in G.state_dict().items()}, 'rng': G.attention.rng.clone()}
+
+    (le, se), (lg, sg) = run(False), run(True)
+    assert [d for _, d in le] == [d for _, d in lg]
+    assert all(torch.equal(se[k], sg[k]) for k in se)
+    assert int(se['rng'][1]) == (9 if dropout else 0)             # 7 critic steps and 2 generator steps
+
+
+def _step(ops, t, cu, rope, pos, leaves, grad):
+    q, k, v, w = leaves
+    a, b = ops.qk_norm_rope(q, k, pos, rope, w, w)
+    o = ops.attention(a, b, v, cu, len_k=t['len'], causal=True)
+    y = ops.dropout_add(o, q, 0.2, t['rng'])
+    return [y.detach()] + list(torch.autograd.grad(y, leaves, grad))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_operators_from_one_graph(dev, dtype):
+    """Forward and backward of the three operators in a captured graph: replayed with other values, lengths and random numbers
+    in the same memory, with eager work in between, every replay gives the eager bits."""
+    from semantic_pyramid_for_image_generation_amd import ops
+    gen = torch.Generator(device=dev).manual_seed(0)
+    T, hq, hk, dim = 200, 4, 2, 64
+    rope = ops.AxialRope((16, 16)); rope.table(dev)
+    pos = torch.randint(0, 100, (T, 2), generator=gen, device=dev, dtype=torch.int32)
+    cu = torch.tensor([0, 70, 70, 190], dtype=torch.int32, device=dev)
+    t = {'len': torch.tensor([70, 0, 100], dtype=torch.int32, device=dev), 'rng': torch.tensor([1, 2], device=dev)}
+    rand = lambda *s: torch.randn(*s, generator=gen, device=dev).to(dtype)
+    src = [rand(T, hq, dim), rand(T, hk, dim), rand(T, hk, dim), rand(dim)]
+    grad = rand(T, hq, dim)
+
+    def fresh():
+        return [s.detach().requires_grad_() for s in src]
+
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        _step(ops, t, cu, rope, pos, fresh(), grad)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    leaves = fresh()
+    with torch.cuda.graph(g):
+        out = _step(ops, t, cu, rope, pos, leaves, grad)
+    for i, bounds in enumerate(([0, 70, 70, 190], [0, 1, 130, 200], [0, 200, 200, 200], [0, 0, 0, 0])):
+        for s in src + [grad]:
+            s.copy_(rand(*s.shape))
+        cu.copy_(torch.tensor(bounds, dtype=torch.int32))
+        t['len'].copy_(torch.tensor([bounds[1], (bounds[2] - bounds[1]) // 2, bounds[3] - bounds[2]], dtype=torch.int32))
+        t['rng'].copy_(torch.tensor([i, 5 * i]))
+        want = _step(ops, t, cu, rope, pos, fresh(), grad)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), (i, bounds)
+        _step(ops, t, cu, rope, pos, fresh(), grad)               # eager work between the replays
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), (i, bounds)
+
+
+def test_two_graphs_and_two_streams(dev):
+    """Two captured token passes (their workspaces are the graphs') replayed side by side, and eager calls on two streams: no
+    state is shared."""
+    from semantic_pyramid_for_image_generation_amd import ops
+    gen = torch.Generator(device=dev).manual_seed(0)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=dev).bfloat16()
+    cu_q = torch.arange(0, 5, dtype=torch.int32, device=dev)
+    cu_k = torch.arange(0, 5 * 3000, 3000, dtype=torch.int32, device=dev)
+    sets = [(rand(4, 8, 128), rand(12000, 2, 128), rand(12000, 2, 128)) for _ in range(2)]
+    call = lambda s: ops.attention(*s, cu_q, cu_k, causal=True)
+    want = [call(s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for _ in range(5):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        eager = []
+        for s, x in zip(streams, sets):
+            with torch.cuda.stream(s):
+                eager.append(call(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, want))
+
+
+def test_rope_table_inside_a_capture_is_refused(dev):
+    from semantic_pyramid_for_image_generation_amd import ops
+    rope = ops.AxialRope((4,))
+    x = torch.randn(2, 1, 8, device=dev)
+    pos = torch.zeros(2, dtype=torch.int32, device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(ops._lib.SempyrError, match="capture"):
+            ops.qk_norm_rope(x, x, pos, rope)
+        x + 1
+    rope.table(dev)
+    ops.qk_norm_rope(x, x, pos, rope)
