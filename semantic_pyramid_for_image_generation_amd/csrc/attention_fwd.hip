@@ -93,17 +93,20 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_wa
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[b][i]);
         mx = half_max(mx);
+        float factor = 1.f;
         if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {                // (never for NaN; a row without a key: -inf > slack)
             const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
             const float alpha = score_exp<T>(m, p.scale_log2, moved);
             m = top;
             base = moved;
             l *= alpha;
-#pragma unroll
-            for (int b = 0; b < DPAD / 32; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
+            factor = alpha;
         }
+        // (multiplied always: under the branch the compiler copies the sums on the other way, 6 % of the time)
+#pragma unroll
+        for (int b = 0; b < DPAD / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] *= factor;
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_wa
                 for (int i = 0; i < 16; ++i) acc[b][i] += part[i];
             }
         } else {
-Frag pf;
+            Frag pf;
             pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::col(vt, cbase, i % (DPAD / 32), i / (DPAD / 32)); }, [&](int i, Frag f) {
                 const int k = i / (DPAD / 32), b = i % (DPAD / 32);
                 if (b == 0) pf = frag_of<T>(sc[k / 2], k % 2);
