@@ -24,7 +24,8 @@ template <typename T, int DPAD> struct KeyTile {
     static constexpr int WAVES_SIMD = DPAD <= 64 ? 2 : 1;               // by registers: heads of 128 need more than 256
 };
 
-template <typename T, int DPAD>
+// REST: see rest_of().
+template <typename T, int DPAD, bool REST>
 __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD((KeyTile<T, DPAD>::WAVES_SIMD)) void attention_dkdv_kernel(Params p)
 {
     typedef KeyTile<T, DPAD> Kt;
@@ -127,13 +128,21 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
             for (int i = 0; i < 16; ++i)
                 if (ki > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[i] = dp[i] = 0.f;
         }
-        Frag pf, df;
+        Frag pf, df, pr, dr;
         pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::col(i % 2 ? qt : ot, cbase, i / 2 % (DPAD / 32), i / 2 / (DPAD / 32)); },
                                             [&](int i, Frag f) {
             const int c = i / 2 % (DPAD / 32), k = i / 2 / (DPAD / 32);
-            if (c == 0 && i % 2 == 0) { pf = frag_of<T>(sc, k); df = frag_of<T>(dp, k); }
+            if (c == 0 && i % 2 == 0) {
+                pf = frag_of<T>(sc, k);
+                df = frag_of<T>(dp, k);
+                if constexpr (REST) { pr = rest_of<T>(sc, pf, k); dr = rest_of<T>(dp, df, k); }
+            }
             if (i % 2) dk[c] = Elem<T>::mma(f, df, dk[c]);
             else dv[c] = Elem<T>::mma(f, pf, dv[c]);
+            if constexpr (REST) {
+                if (i % 2) dk[c] = Elem<T>::mma(f, dr, dk[c]);
+                else dv[c] = Elem<T>::mma(f, pr, dv[c]);
+            }
         });
     }
 
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
 }
 
 // delta and dQ: as the forward, with dO beside Q in registers and K read by columns, too.
-template <typename T, int DPAD>
+template <typename T, int DPAD, bool REST>
 __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIMD((sizeof(T) * DPAD <= 256 ? 2 : 1)) void attention_dq_kernel(Params p)
 {
     typedef Tile<T, DPAD, BN> Tl;
@@ -278,11 +287,15 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIM
                     acc[c] += part;
                 }
             } else {
-                Frag df;
+                Frag df, dr;
                 pipelined<Frag, DPAD / 16, BATCH<T>>([&](int i) { return Tl::col(kt, cbase, i % (DPAD / 32), n * 2 + i / (DPAD / 32)); }, [&](int i, Frag f) {
                     const int c = i % (DPAD / 32);
-                    if (c == 0) df = frag_of<T>(dp, i / (DPAD / 32));
+                    if (c == 0) {
+                        df = frag_of<T>(dp, i / (DPAD / 32));
+                        if constexpr (REST) dr = rest_of<T>(dp, df, i / (DPAD / 32));
+                    }
                     acc[c] = Elem<T>::mma(f, df, acc[c]);
+                    if constexpr (REST) acc[c] = Elem<T>::mma(f, dr, acc[c]);
                 });
             }
         }
@@ -303,13 +316,18 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIM
 }
 
 // Instantiated by name: this compiler's host pass leaves the stubs of the implicit instantiations out.
-#define SEMPYR_BWD_KERNELS(T, D) template __global__ void attention_dkdv_kernel<T, D>(Params); template __global__ void attention_dq_kernel<T, D>(Params);
-SEMPYR_BWD_KERNELS(float, 32) SEMPYR_BWD_KERNELS(float, 64) SEMPYR_BWD_KERNELS(float, 128)
-SEMPYR_BWD_KERNELS(f16, 32) SEMPYR_BWD_KERNELS(f16, 64) SEMPYR_BWD_KERNELS(f16, 128)
-SEMPYR_BWD_KERNELS(bf16, 32) SEMPYR_BWD_KERNELS(bf16, 64) SEMPYR_BWD_KERNELS(bf16, 128)
+#define SEMPYR_BWD_KERNELS(T, D, R) \
+    template __global__ void attention_dkdv_kernel<T, D, R>(Params); template __global__ void attention_dq_kernel<T, D, R>(Params);
+#define SEMPYR_BWD_DIMS(T, R) SEMPYR_BWD_KERNELS(T, 32, R) SEMPYR_BWD_KERNELS(T, 64, R) SEMPYR_BWD_KERNELS(T, 128, R)
+SEMPYR_BWD_DIMS(float, false)
+SEMPYR_BWD_DIMS(f16, false)
+SEMPYR_BWD_DIMS(f16, true)
+SEMPYR_BWD_DIMS(bf16, false)
+SEMPYR_BWD_DIMS(bf16, true)
+#undef SEMPYR_BWD_DIMS
 #undef SEMPYR_BWD_KERNELS
 
-template <typename T, int DPAD>
+template <typename T, int DPAD, bool REST>
 static int launch_bwd_d(const Params& p, hipStream_t st) {
     typedef KeyTile<T, DPAD> Kt;
     const int64_t bk = work_blocks(num_tiles(p.nseq, p.total_k, Kt::KEYS), p.heads_k, 1);
@@ -317,29 +335,33 @@ static int launch_bwd_d(const Params& p, hipStream_t st) {
     if (bk > 0x7FFFFFFF || bq > 0x7FFFFFFF) SEMPYR_FAIL("attention_bwd: too many tiles");
     const int lds_q = stages_of<T, DPAD>() * 2 * Tile<T, DPAD, BN>::BYTES;
     if (p.total_q > 0) {
-        if (int rc = allow_lds((const void*)attention_dq_kernel<T, DPAD>, lds_q)) return rc;
-        attention_dq_kernel<T, DPAD><<<(unsigned)bq, 256, lds_q, st>>>(p);
+        if (int rc = allow_lds((const void*)attention_dq_kernel<T, DPAD, REST>, lds_q)) return rc;
+        attention_dq_kernel<T, DPAD, REST><<<(unsigned)bq, 256, lds_q, st>>>(p);
         SEMPYR_CHECK_LAUNCH();
     }
     if (p.total_k > 0) {
-        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD>, Kt::LDS)) return rc;
-        attention_dkdv_kernel<T, DPAD><<<(unsigned)bk, 256, Kt::LDS, st>>>(p);
+        if (int rc = allow_lds((const void*)attention_dkdv_kernel<T, DPAD, REST>, Kt::LDS)) return rc;
+        attention_dkdv_kernel<T, DPAD, REST><<<(unsigned)bk, 256, Kt::LDS, st>>>(p);
         SEMPYR_CHECK_LAUNCH();
     }
     return 0;
 }
 
-template <typename T>
+template <typename T, bool REST>
 static int launch_bwd_t(const Params& p, hipStream_t st) {
-    if (p.dim <= 32) return launch_bwd_d<T, 32>(p, st);
-    if (p.dim <= 64) return launch_bwd_d<T, 64>(p, st);
-    return launch_bwd_d<T, 128>(p, st);
+    if (p.dim <= 32) return launch_bwd_d<T, 32, REST>(p, st);
+    if (p.dim <= 64) return launch_bwd_d<T, 64, REST>(p, st);
+    return launch_bwd_d<T, 128, REST>(p, st);
 }
 
 int launch_bwd(int dtype, const Params& p, hipStream_t st) {
-    if (dtype == SEMPYR_F32) return launch_bwd_t<float>(p, st);
-    if (dtype == SEMPYR_F16) return launch_bwd_t<f16>(p, st);
-    return launch_bwd_t<bf16>(p, st);
+    // Rounding P and dS to 16 bits adds as much error as the results' own rounding.  Over many keys that evens out at 1.4
+    // times the latter; a few short sequences can come out worse, and there -- less than a workgroup of 32 keys a CU, waiting
+    // for memory and launches anyway -- the rest is multiplied, too (REST_TIMES).
+    const bool rest = (int64_t)p.total_k * p.heads_k <= 8192;
+    if (dtype == SEMPYR_F32) return launch_bwd_t<float, false>(p, st);
+    if (dtype == SEMPYR_F16) return rest ? launch_bwd_t<f16, true>(p, st) : launch_bwd_t<f16, false>(p, st);
+    return rest ? launch_bwd_t<bf16, true>(p, st) : launch_bwd_t<bf16, false>(p, st);
 }
 
 }  // namespace attn

@@ -5,7 +5,7 @@
 // waves of a workgroup.  A wave streams its tiles through an LDS ring of its own (no barrier in the loop, one tile in flight
 // while one is used) and keeps a running maximum and sum; the waves' results are joined in LDS, those of the workgroups by a
 // second kernel from fp32 partial sums.  Bound by reading K and V; the matrix pipe has most of its columns idle for a single
-// token, which costs nothing here.
+// token and time to spare: it also takes what rounding the probabilities to 16 bits leaves (no difference in time).
 #include "attn_tile.h"
 #include "attention.h"
 
@@ -126,9 +126,13 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
         l += sum;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const Frag pf = frag_of<T>(sc, k);
+            const Frag pf = frag_of<T>(sc, k), pr = rest_of<T>(sc, pf, k);
 #pragma unroll
-            for (int c = 0; c < DPAD / 32; ++c) acc[c] = Elem<T>::mma(Tl::col(vt, cbase, c, k), pf, acc[c]);
+            for (int c = 0; c < DPAD / 32; ++c) {
+                const Frag f = Tl::col(vt, cbase, c, k);
+                acc[c] = Elem<T>::mma(f, pf, acc[c]);
+                if constexpr (sizeof(T) == 2) acc[c] = Elem<T>::mma(f, pr, acc[c]);
+            }
         }
     }
     l = half_sum(l);

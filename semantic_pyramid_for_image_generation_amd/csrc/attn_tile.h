@@ -69,6 +69,16 @@ __device__ __forceinline__ typename Elem<T>::Frag frag_of(const f32x16& s, int t
     return f;
 }
 
+// what that rounding took: added as a second product where the matrix pipe has the time, it makes the operand exact to twice
+// the type's bits
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Frag rest_of(const f32x16& s, const typename Elem<T>::Frag& f, int t) {
+    typename Elem<T>::Frag r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)(s[t * 8 + j] - (float)f[j]);
+    return r;
+}
+
 // ---------------------------------------------------------------------------------------------- tiles
 template <typename T, int DPAD, int ROWS>
 struct Tile {
