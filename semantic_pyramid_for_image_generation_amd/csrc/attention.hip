@@ -9,7 +9,7 @@ int fill_params(const sempyr_attention_desc* d, attn::Params& p, const char* who
     const int sz = dtype_size(d->dtype);
     if (d->dim < 1 || d->dim > 128 || d->dim * sz % 16) SEMPYR_FAIL("%s: head dim must be at most 128 and whole 16-byte vectors, got %d", who, d->dim);
     if (d->heads_q < 1 || d->heads_k < 1 || d->heads_q > 65536 || d->heads_q % d->heads_k) SEMPYR_FAIL("%s: %d query heads over %d key heads", who, d->heads_q, d->heads_k);
-    if (d->total_q < 0 || d->total_k < 0 || d->total_q > 0x7FFFFF00 || d->total_k > 0x7FFFFF00) SEMPYR_FAIL("%s: %lld / %lld rows", who, (long long)d->total_q, (long long)d->total_k);
+    if (d->total_q < 0 || d->total_k < 0 || d->total_q > 1 << 30 || d->total_k > 1 << 30) SEMPYR_FAIL("%s: %lld / %lld rows", who, (long long)d->total_q, (long long)d->total_k);
     if (d->nseq < 0 || d->nseq > 1 << 24) SEMPYR_FAIL("%s: %d sequences", who, d->nseq);
     if (!(d->scale > 0.f) || !(d->scale < INFINITY)) SEMPYR_FAIL("%s: scale must be positive and finite", who);
     const int64_t strides[] = {d->q_stride_token, d->k_stride_token, d->v_stride_token, d->q_stride_head, d->k_stride_head, d->v_stride_head};

@@ -137,6 +137,11 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_wa
     }
     for (; t < tiles; ++t, b = b + 1 == STAGES ? 0 : b + 1) turn(t);
     wait_loads<0>();
+    if (p.causal && !finite_in_wave(acc, present)) {
+#pragma unroll
+        for (int b = 0; b < DPAD / 32; ++b) acc[b] = f32x16{};
+        sum_seen<T, DPAD>(acc, qf, kbase, vbase, p, 0, min(sq.lk, max(see_wave, 0)), see, base, lane);
+    }
     l = half_sum(l);                                 // each lane half has summed its own keys
     if (!present) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;      // no key: zeros

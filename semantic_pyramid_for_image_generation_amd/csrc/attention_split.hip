@@ -135,6 +135,11 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
             }
         }
     }
+    if (p.causal && !finite_in_wave(acc, present)) {
+#pragma unroll
+        for (int c = 0; c < DPAD / 32; ++c) acc[c] = f32x16{};
+        for (int t = t0; t < t1; t += WAVES) sum_seen<T, DPAD>(acc, qf, kbase, vbase, p, t * BK, min(sq.lk, (t + 1) * BK), see, base, lane);
+    }
     l = half_sum(l);
 
     // join the waves: [wave][column][dim] in LDS, every thread then owns four elements of a column

@@ -406,6 +406,46 @@ __device__ __forceinline__ Where locate(const Params& p, int number, int R, int 
 // numbers that have to be launched: the exact count is only known on the device
 __host__ __device__ inline int num_tiles(int nseq, int total, int R) { return total / R + nseq + 1; }
 
+// Sums p V over keys k0 .. k1 - 1 without the matrix pipe, each query (lane pair) over the keys it sees and no others.  A product
+// of a hidden key's probability, 0, with a NaN or an infinity in its V row would be NaN: where a sum is not finite, a causal
+// wave redoes it with this.  Slow (a dot product a key), and only ever run on such input.
+template <typename T, int DPAD>
+__device__ __forceinline__ void sum_seen(f32x16 (&acc)[DPAD / 32], const typename Elem<T>::Frag (&qf)[DPAD / 16], const T* kbase, const T* vbase,
+                                         const Params& p, int k0, int k1, int see, float base, int lane) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    const int half = lane >> 5;
+    for (int k = k0; k < k1; ++k) {
+        typename Elem<T>::Frag kf[DPAD / 16];
+        load_row_frags<T, DPAD>(kf, kbase + (int64_t)k * p.k_tok, true, p.dim, lane);
+        float s = 0.f;
+#pragma unroll
+        for (int d = 0; d < DPAD / 16; ++d)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf((float)qf[d][j], (float)kf[d][j], s);
+        const float e = score_exp<T>(half_sum(s), p.scale_log2, base);
+#pragma unroll
+        for (int b = 0; b < DPAD / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = b * 32 + r * 8 + half * 4;
+                if (d >= p.dim) continue;
+                const V4 v = *reinterpret_cast<const V4*>(vbase + (int64_t)k * p.v_tok + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[b][r * 4 + i] = k < see ? fmaf(e, (float)v[i], acc[b][r * 4 + i]) : acc[b][r * 4 + i];
+            }
+    }
+}
+template <int N>
+__device__ __forceinline__ bool finite_in_wave(const f32x16 (&acc)[N], bool present) {
+    float x = 0.f;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x = fmaf(acc[b][i], 0.f, x);
+    return !__any(present && x != 0.f);              // (0 times an infinity or a NaN is NaN)
+}
+
 // Workgroup -> (tile number, kv head, head in group).  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: an XCD
 // gets whole kv heads where there are enough, else every X-th tile of one, so that K and V of a head are read into few L2s;
 // within an XCD the heads of a group come next to each other.

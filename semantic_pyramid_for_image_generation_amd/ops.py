@@ -2065,7 +2065,8 @@ def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
     cu_k[s] .. cu_k[s + 1] - 1 (cu_k None: cu_q), of which the first len_k[s] count (None: all); int32 tensors on the device,
     the first entry of a table is 0.  causal: the last query sees all keys, the one before it one less, and so on.  Queries
     that see no key give zeros, as do rows behind the last sequence; keys that nobody sees get zero gradients, and what lies
-    in rows behind len_k[s] is never read.  scale None: dim ** -0.5.  dim: a multiple of 8 (fp32: 4) up to 128.
+    in rows behind len_k[s] is never read.  A NaN or an infinity in a sequence's own keys reaches the queries that see it (in the
+    backward pass it may reach the gradients of the whole sequence).  scale None: dim ** -0.5.  dim: a multiple of 8 (fp32: 4) up to 128.
     Differentiable in q, k and v; the sums of both passes have a fixed order."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2] or 0 in q.shape[1:] or 0 in k.shape[1:] or \
             q.shape[1] % k.shape[1]:
@@ -2074,8 +2075,8 @@ def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
     unit = 16 // q.element_size()
     if q.shape[2] % unit or q.shape[2] > 128:
         raise _lib.SempyrError(f"attention: a head dim that is a multiple of {unit}, at most 128, expected, got {q.shape[2]}")
-    if max(q.shape[0], k.shape[0]) > 0x7FFFFF00:
-        raise _lib.SempyrError("attention: more than 2^31 rows")
+    if max(q.shape[0], k.shape[0]) > 2 ** 30:
+        raise _lib.SempyrError("attention: more than 2^30 rows")
     if cu_k is None:
         if q.shape[0] != k.shape[0]:
             raise _lib.SempyrError("attention: cu_k is needed where queries and keys differ in number")

@@ -170,3 +170,33 @@ def test_attention_second_order_refused(ops, dev):
     q = torch.randn(5, 1, 16, device=dev, requires_grad=True)
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(ops.attention(q, q, q, table([5], dev)).square().sum(), q, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,heads", [([100], 2), ([130] * 9, 64)])          # split over keys; one pass
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_attention_hidden_nan(ops, dev, lens, heads, dtype, bad):
+    """A NaN or an infinity in a key or value that the causal mask hides leaves the queries before it alone, to the bit where no
+    tile has to be redone, and within the tolerance where it has; queries that see it get what the definition gives."""
+    gen = torch.Generator().manual_seed(9)
+    T = sum(lens)
+    q, k, v = (torch.randn(T, h, 32, generator=gen).to(dtype) for h in (heads, heads // 2, heads // 2))
+    spans_ = spans(lens, lens, lens)
+    (w, e), *_ = oracle.attention(q, k, v, torch.zeros_like(q), spans_[:1], True, 32 ** -0.5)
+    at = 40                                                                   # of the first sequence
+    clean = ops.attention(q.to(dev), k.to(dev), v.to(dev), table(lens, dev), causal=True)
+    for which in (0, 1):
+        kb, vb = k.clone(), v.clone()
+        (kb if which == 0 else vb)[at, 0, 3] = bad
+        o = ops.attention(q.to(dev), kb.to(dev), vb.to(dev), table(lens, dev), causal=True)
+        within(o[:at], w[:at], e[:at], f"before {which}")
+        assert torch.equal(o[lens[0]:], clean[lens[0]:]) and torch.equal(o[:, 2:], clean[:, 2:])
+        seen = o[at:lens[0], :2].float().cpu()
+        if which == 1:
+            col = seen[:, :, 3]
+            assert not torch.isfinite(col).any()
+            if bad != bad or dtype == torch.float32:
+                assert torch.isnan(col).all() if bad != bad else (col == bad).all()
+            within(o[at:lens[0], :2, 4:], w[at:lens[0], :2, 4:], e[at:lens[0], :2, 4:], "other columns")
+        elif bad != bad:
+            assert torch.isnan(seen).all()
