@@ -4,7 +4,7 @@ the reference's."""
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import ops, parallel
 from .blocks import init_weights, run_conv, run_norm
 
 
@@ -59,7 +59,8 @@ class SelfAttention2d(nn.Module):
         o = run_conv(self.proj, o.view(B, H * W, C).transpose(1, 2).reshape(B, C, H, W))
         if self.dropout == 0.0 or not self.training:
             return ops.add_act(x, o)
-        # the backward pass needs this pass's offset (an addition, not a copy: the loop's graph replay takes kernels)
-        now = self.rng + 0
+        # the backward pass needs this pass's offset (an addition and no copy: the loop's graph replay
+        # takes kernels only)
+        now = self.rng + parallel.rank()    # ranks hold equal state and other samples: other decisions, too
         self.rng[1].add_(1)
         return ops.dropout_add(o, x, self.dropout, now)

@@ -2,13 +2,18 @@
 //
 // A workgroup owns 128 queries of one head, a wave 32 of them (a query = a lane pair, see attn_tile.h).  Per tile of 64 keys:
 //     S^T = K Q^T, P = exp2(c S - c m), l += sum P, O^T += V^T P
-// with c = scale log2(e) and a reference m that follows the maximum in steps (l and O^T are rescaled when it moves).  Queries and the output accumulator stay in registers; K and V tiles come through a ring in
-// LDS, the next tiles' DMA runs under the current tile's products.
+// with c = scale log2(e) and a reference m that follows the maximum in steps (l and O^T are rescaled when it moves).  Queries
+// and the output accumulator stay in registers; K and V tiles come through a ring in LDS, the next tiles' DMA runs under the
+// current tile's products.
+//
+// 16384 tokens, 16/2 heads of 128, causal, fp16: 1.14 ms, 960 TFLOP/s, 86 % of what an 8192^3 library product reaches.  Bound
+// by the matrix and the vector pipe in turn -- counters: 524 k of 1180 k cycles MFMA, about as many vector instructions, LDS
+// waits 5 %, no bank conflicts -- at a clock that the load takes down to 1.9 GHz.  fp32 (16 x 1024 tokens, 2 heads of 64, 88 us):
+// MFMA 62 % busy, one wave a SIMD.
 #include "attn_tile.h"
 #include "attention.h"
 
 namespace attn {
-
 
 // waves a SIMD holds, by registers
 template <typename T, int DPAD> constexpr int fwd_waves() { return sizeof(T) * DPAD <= 128 ? 3 : sizeof(T) * DPAD <= 256 ? 2 : 1; }

@@ -145,16 +145,18 @@ __device__ __forceinline__ BufferDesc buffer_desc(const void* base, int bytes) {
                       __builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
 __device__ __forceinline__ unsigned lds_offset(const void* p) { return (unsigned)(uintptr_t)(LDS_PTR const char*)p; }
+// s_nop 4: five wait states, should the compiler have written the descriptor with a vector instruction right before (it does not
+// look for that hazard into assembly); m0 needs one.
 // (m0, the DMA's LDS address, is a reserved register: the compiler warns that it does not keep a value there across the block,
 // which is what the clobber says)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(BufferDesc rsrc, int offset, const void* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(lds_offset(lds))), "v"(offset), "s"(rsrc) : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(BufferDesc rsrc, int offset, const void* lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(lds_offset(lds))), "v"(offset), "s"(rsrc) : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -396,6 +398,7 @@ __device__ __forceinline__ Where locate(const Params& p, int number, int R, int 
         const int rank = above + r - (upto - mine);                      // in its sequence, by falling load
         w.row = __builtin_amdgcn_readlane(!BY_KEYS && p.causal ? n - 1 - rank : rank, w.s) * R;
     }
+    w.ok = w.row >= 0 && w.row < __builtin_amdgcn_readlane(rows, w.s);       // (always, unless the table's entries fall)
     w.sq.q0 = __builtin_amdgcn_readlane(sq.q0, w.s);
     w.sq.lq = __builtin_amdgcn_readlane(sq.lq, w.s);
     w.sq.k0 = __builtin_amdgcn_readlane(sq.k0, w.s);

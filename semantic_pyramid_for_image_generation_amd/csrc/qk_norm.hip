@@ -13,7 +13,9 @@
 // Bound by memory: x is read once and y written once (and g, dx).  A group of 2^k lanes owns a row (token, head); a lane holds
 // PAIRS pairs, that is two 16-byte vectors, in such a way that both halves of every pair lie in the same lane, in either pair
 // order -- the rotation needs no exchange, the norm k shuffles.  A group walks over a slice of the token's heads with the
-// sines and cosines of its pairs in registers.
+// sines and cosines of its pairs in registers.  32768 tokens, 32 + 8 heads of 128, bf16, forward: 671 MB in 138 us (4.9 TB/s,
+// 94 % of a copy's rate); 16196 tokens, 16 + 4 heads of 96, fp16: forward 35 us, backward 63 + 4 us (a group of 8 lanes has
+// 2 idle at 96).
 #include "tokens.h"
 
 namespace {

@@ -1907,9 +1907,11 @@ class AxialRope:
 
     def table(self, device):
         device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", _cur_device())
         t = self._tables.get(device)
         if t is None:
-            if torch.cuda.is_current_stream_capturing():
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise _lib.SempyrError("AxialRope: first use on this device during a graph capture; call table(device) before it")
             signed = [f - 2 ** 64 if f >= 2 ** 63 else f for f in self.fractions()]
             t = self._tables[device] = torch.tensor(signed, dtype=torch.int64).to(device)
@@ -1999,18 +2001,25 @@ def qk_norm_rope(q, k, positions, rope, q_weight=None, k_weight=None, eps=1e-6):
 
 
 def _attn_rows(t):
-    """t as the kernels read it: unit stride in the last dimension, rows on 16 bytes, token stride at least a row (an expanded
-    dimension has none) and below 2^23 elements; anything else is copied."""
+    """(t, token stride, head stride) as the kernels read it: unit stride in the last dimension, rows on 16 bytes, token stride
+    at least a row (an expanded dimension has none) and below 2^23 elements; anything else is copied.  Strides of dimensions
+    of size one mean nothing and are replaced."""
     unit = 16 // t.element_size()
-    st, sh, sd = t.stride()
-    if sd != 1 or st % unit or sh % unit or t.data_ptr() % 16 or st < t.shape[2] or st > 2 ** 23:
+    (rows, heads, dim), (st, sh, sd) = t.shape, t.stride()
+    if rows <= 1:
+        st = heads * dim
+    if heads == 1:
+        sh = dim
+    if sd != 1 or st % unit or sh % unit or t.data_ptr() % 16 or st < dim or st > 2 ** 23:
         t = t.contiguous()
-        return t if t.data_ptr() % 16 == 0 else t.clone()
-    return t
+        t = t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+        st, sh = heads * dim, dim
+    return t, st, sh
 
 
 def _attn_desc(q, k, v, nseq, causal, scale, dtype):
-    (total_q, heads_q, dim), (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.shape, q.stride(), k.stride(), v.stride()
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = q, k, v
+    total_q, heads_q, dim = q.shape
     return _lib.AttentionDesc(total_q, k.shape[0], qt, qh, kt, kh, vt, vh, dtype, heads_q, k.shape[1], dim, nseq, causal, scale)
 
 
@@ -2026,7 +2035,8 @@ class _Attention(Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, len_k, causal, scale, dtype):
         with _on_device(q.device):
-            q, k, v = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+            rows = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+            q, k, v = (r[0] for r in rows)
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
             len_k = len_k if len_k is None else len_k.contiguous()
             o = q.new_empty(q.shape)
@@ -2034,7 +2044,7 @@ class _Attention(Function):
             if any(ctx.needs_input_grad[:3]):
                 stats = torch.empty((2 if dtype == _lib.F32 else 1, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
                 low = torch.empty_like(o) if dtype != _lib.F32 else None
-            desc = ctypes.byref(_attn_desc(q, k, v, cu_q.numel() - 1, causal, scale, dtype))
+            desc = ctypes.byref(_attn_desc(*rows, cu_q.numel() - 1, causal, scale, dtype))
             n = _attn_workspace(q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], cu_q.numel() - 1, dtype)
             ws = _workspace(4 * n, q.device)
             check(L.sempyr_attention_fwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k),
@@ -2050,7 +2060,7 @@ class _Attention(Function):
         q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
         with _on_device(q.device):
             g = g.contiguous()
-            g = g if g.data_ptr() % 16 == 0 else g.clone()
+            g = g if g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             delta = torch.empty_like(stats[0])
             check(L.sempyr_attention_bwd(ctx.cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(), cu_q.data_ptr(),

@@ -108,6 +108,18 @@ def test_attention_views(ops, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_attention_dimensions_of_size_one(ops, dev, dtype):
+    """Their strides mean nothing: one row, one head, from views whose strides there are odd or zero."""
+    x = torch.randn(5, 3, 33, device=dev).to(dtype)
+    cu1, cu5 = table([1], dev), table([5], dev)
+    one_row = torch.as_strided(x.contiguous()[:1, :, :32].clone(), (1, 3, 32), (3, 32, 1))
+    one_head = torch.as_strided(x[:, :1, :32].contiguous(), (5, 1, 32), (32, 5, 1))
+    for q, cu in ((one_row, cu1), (one_head, cu5)):
+        o = ops.attention(q, q, q, cu, causal=True)
+        assert torch.equal(o, ops.attention(*[q.clone(memory_format=torch.contiguous_format)] * 3, cu, causal=True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_large_scores(ops, dev, dtype):
     """Scores in the hundreds: the running maximum keeps every exponential in range."""
     gen = torch.Generator().manual_seed(2)

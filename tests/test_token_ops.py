@@ -35,6 +35,12 @@ def test_rope_fractions(ops, sections, shared):
             assert abs(math.cos(2 * math.pi * wrapped) - math.cos(pos * f)) <= 2.0 ** -52 * max(1, abs(pos)) * 8
 
 
+def test_rope_table_on_the_host(ops):
+    rope = ops.AxialRope((5, 0, 3))
+    t = rope.table("cpu")
+    assert t.dtype == torch.int64 and [int(v) % 2 ** 64 for v in t] == rope.fractions() and rope.table(torch.device("cpu")) is t
+
+
 def test_rope_refusals(ops):
     E = ops._lib.SempyrError
     for bad in ((), (0,), (-1, 4), (1,) * 5):
