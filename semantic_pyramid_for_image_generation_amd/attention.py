@@ -37,15 +37,21 @@ class SelfAttention2d(nn.Module):
 
     def _grid(self, B, H, W, device):
         """(positions, sequence table) of B maps; kept per shape, except under a graph capture, whose memory is the graph's."""
+        capturing = device.type == 'cuda' and torch.cuda.is_current_stream_capturing()
         key = (B, H, W, device)
         hit = self._places.get(key)
         if hit is None:
-            i = torch.arange(B * H * W, device=device, dtype=torch.int32)
-            hit = (torch.stack([i // W % H, i % W], dim=1).to(torch.int32),
-                   torch.arange(0, (B + 1) * H * W, H * W, device=device, dtype=torch.int32))
-            if not torch.cuda.is_current_stream_capturing():
+            # kept ones are made on the host: their copy has ended when it returns, so any stream may use them next
+            where = device if capturing else torch.device('cpu')
+            i = torch.arange(B * H * W, device=where, dtype=torch.int32)
+            hit = (torch.stack([i // W % H, i % W], dim=1).to(device, torch.int32),
+                   torch.arange(0, (B + 1) * H * W, H * W, device=where, dtype=torch.int32).to(device))
+            if not capturing:
                 self._places[key] = hit
         return hit
+
+    def __getstate__(self):
+        return dict(self.__dict__, _places={})
 
     def forward(self, x):
         B, C, H, W = x.shape
@@ -59,8 +65,8 @@ class SelfAttention2d(nn.Module):
         o = run_conv(self.proj, o.view(B, H * W, C).transpose(1, 2).reshape(B, C, H, W))
         if self.dropout == 0.0 or not self.training:
             return ops.add_act(x, o)
-        # the backward pass needs this pass's offset (an addition and no copy: the loop's graph replay
-        # takes kernels only)
-        now = self.rng + parallel.rank()    # ranks hold equal state and other samples: other decisions, too
+        # The backward pass needs this pass's offset (an addition and no copy: the loop's graph replay takes kernels only).
+        # Ranks hold equal state and other samples: their decisions differ, too.
+        now = self.rng + parallel.rank()
         self.rng[1].add_(1)
         return ops.dropout_add(o, x, self.dropout, now)

@@ -1894,6 +1894,9 @@ class AxialRope:
         self._tables = {}
         self._sections_c = (ctypes.c_int32 * 4)(*self.sections)
 
+    def __reduce__(self):                              # copies and pickles carry the settings, not the device tables
+        return AxialRope, (self.sections, self.base, self.interleaved, self.shared)
+
     def frequencies(self):
         """The angle of one position step, per pair (radians)."""
         if self.shared:

@@ -44,3 +44,26 @@ def test_flags():
     assert e.attention_size == 16
     with pytest.raises(SystemExit):
         train_model.build_parser().parse_args(['--attention-size', '10'])
+
+
+def test_copies_and_pickles():
+    import copy
+    import pickle
+    from semantic_pyramid_for_image_generation_amd import ops
+    from semantic_pyramid_for_image_generation_amd.generator import Generator
+    g = Generator('res', attention_size=16)
+    g.attention._grid(2, 3, 5, torch.device('cpu'))
+    for other in (copy.deepcopy(g), pickle.loads(pickle.dumps(g))):
+        assert all(torch.equal(a, b) for a, b in zip(g.state_dict().values(), other.state_dict().values()))
+        assert torch.equal(g.attention.rng, other.attention.rng) and other.attention._places == {}
+    r = ops.AxialRope((3, 0, 5), base=77.0, interleaved=True, shared=True)
+    for other in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert (other.sections, other.base, other.interleaved, other.shared) == ((3, 0, 5), 77.0, True, True)
+        assert torch.equal(other.table('cpu'), r.table('cpu')) and list(other._sections_c) == [3, 0, 5, 0]
+
+
+def test_places_of_a_map():
+    from semantic_pyramid_for_image_generation_amd.attention import SelfAttention2d
+    positions, table = SelfAttention2d(64)._grid(2, 3, 5, torch.device('cpu'))
+    assert positions.tolist() == [[y, x] for _ in range(2) for y in range(3) for x in range(5)] and table.tolist() == [0, 15, 30]
+    assert positions.dtype == table.dtype == torch.int32

@@ -68,6 +68,22 @@ def test_block(dev, shape, dropout):
         assert float((blk(xg).double().cpu() - plain).norm()) <= REL * float(plain.norm())
 
 
+def test_ranks_drop_other_elements(dev, monkeypatch):
+    from semantic_pyramid_for_image_generation_amd import parallel
+    from semantic_pyramid_for_image_generation_amd.attention import SelfAttention2d
+    torch.manual_seed(0)
+    blk = SelfAttention2d(64, dropout=0.5).to(dev).train()
+    x = torch.randn(2, 64, 8, 8, device=dev)
+    state, outs = blk.rng.clone(), []
+    for rank in (0, 1, 0):
+        monkeypatch.setattr(parallel, 'rank', lambda rank=rank: rank)
+        blk.rng.copy_(state)
+        with torch.no_grad():
+            outs.append((blk(x) == x).float())             # where the branch was dropped
+    # 8192 fair coins: equal in 4096 places, within 8 standard deviations of 45
+    assert torch.equal(outs[0], outs[2]) and abs(int((outs[0] == outs[1]).sum()) - 4096) < 8 * 45.3
+
+
 @pytest.mark.parametrize("gen_type,size", [('res', 32), ('default', 8)])
 def test_generator_runs_with_attention(dev, gen_type, size):
     from semantic_pyramid_for_image_generation_amd.generator import Generator
