@@ -11,7 +11,8 @@ int fill_params(const sempyr_attention_desc* d, attn::Params& p, const char* who
     if (d->heads_q < 1 || d->heads_k < 1 || d->heads_q > 65536 || d->heads_q % d->heads_k) SEMPYR_FAIL("%s: %d query heads over %d key heads", who, d->heads_q, d->heads_k);
     if (d->total_q < 0 || d->total_k < 0 || d->total_q > 1 << 30 || d->total_k > 1 << 30) SEMPYR_FAIL("%s: %lld / %lld rows", who, (long long)d->total_q, (long long)d->total_k);
     if (d->nseq < 0 || d->nseq > 1 << 24) SEMPYR_FAIL("%s: %d sequences", who, d->nseq);
-    if (!(d->scale > 0.f) || !(d->scale < INFINITY)) SEMPYR_FAIL("%s: scale must be positive and finite", who);
+    // (the kernels multiply by scale log2(e))
+    if (!(d->scale > 0.f) || !(d->scale * 1.4426950408889634f < INFINITY)) SEMPYR_FAIL("%s: scale must be positive and below 2e38", who);
     const int64_t strides[] = {d->q_stride_token, d->k_stride_token, d->v_stride_token, d->q_stride_head, d->k_stride_head, d->v_stride_head};
     for (int i = 0; i < 6; ++i) {
         if (strides[i] < 0 || strides[i] * sz % 16) SEMPYR_FAIL("%s: strides must be whole 16-byte vectors", who);

@@ -333,7 +333,7 @@ static int launch_bwd_d(const Params& p, hipStream_t st) {
     typedef KeyTile<T, DPAD> Kt;
     const int64_t bk = work_blocks(num_tiles(p.nseq, p.total_k, Kt::KEYS), p.heads_k, 1);
     const int64_t bq = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
-    if (bk > 0x7FFFFFFF || bq > 0x7FFFFFFF) SEMPYR_FAIL("attention_bwd: too many tiles");
+    if (!grid_fits(bk, 256) || !grid_fits(bq, 256)) SEMPYR_FAIL("attention_bwd: too many tiles");
     const int lds_q = stages_of<T, DPAD>() * 2 * Tile<T, DPAD, BN>::BYTES;
     if (p.total_q > 0) {
         if (int rc = allow_lds((const void*)attention_dq_kernel<T, DPAD, REST>, lds_q)) return rc;
@@ -358,7 +358,7 @@ static int launch_bwd_t(const Params& p, hipStream_t st) {
 int launch_bwd(int dtype, const Params& p, hipStream_t st) {
     // Rounding P and dS to 16 bits adds as much error as the results' own rounding.  Over many keys that evens out at 1.4
     // times the latter; a few short sequences can come out worse, and there -- less than a workgroup of 32 keys a CU, waiting
-    // for memory and launches anyway -- the rest is multiplied, too (REST_TIMES).
+    // for memory and launches anyway -- the rest is multiplied, too.
     const bool rest = (int64_t)p.total_k * p.heads_k <= 8192;
     if (dtype == SEMPYR_F32) return launch_bwd_t<float, false>(p, st);
     if (dtype == SEMPYR_F16) return rest ? launch_bwd_t<f16, true>(p, st) : launch_bwd_t<f16, false>(p, st);

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_wa
 template <typename T, int DPAD>
 static int launch_fwd_d(const Params& p, hipStream_t st) {
     const int64_t blocks = work_blocks(num_tiles(p.nseq, p.total_q, BM), p.heads_k, p.group);
-    if (blocks > 0x7FFFFFFF) SEMPYR_FAIL("attention_fwd: too many tiles");
+    if (!grid_fits(blocks, 256)) SEMPYR_FAIL("attention_fwd: too many tiles");
     const int bytes = stages_of<T, DPAD>() * 2 * Tile<T, DPAD, BN>::BYTES;
     if (int rc = allow_lds((const void*)attention_fwd_kernel<T, DPAD>, bytes)) return rc;
     attention_fwd_kernel<T, DPAD><<<(unsigned)blocks, 256, bytes, st>>>(p);

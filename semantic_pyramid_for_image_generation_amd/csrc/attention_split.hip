@@ -253,7 +253,7 @@ static int launch_split_d(const Params& p, const SplitPlan& plan, float* ws, hip
     typedef Split<T, DPAD> Sp;
     const int64_t rows = (int64_t)p.total_q * p.heads_q;
     const int64_t blocks = (int64_t)num_tiles(p.nseq, p.total_q, plan.queries) * plan.splits * p.heads_k * plan.head_chunks;
-    if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFF) SEMPYR_FAIL("attention_fwd: too many tiles");
+    if (!grid_fits(blocks, 64 * Sp::WAVES) || (plan.splits > 1 && !grid_fits(rows, 256))) SEMPYR_FAIL("attention_fwd: too many tiles");
     float* ml = ws ? ws + plan.splits * rows * p.dim : nullptr;
     if (int rc = allow_lds((const void*)attention_split_kernel<T, DPAD>, Sp::LDS)) return rc;
     attention_split_kernel<T, DPAD><<<(unsigned)blocks, 64 * Sp::WAVES, Sp::LDS, st>>>(p, plan, ws, ml);

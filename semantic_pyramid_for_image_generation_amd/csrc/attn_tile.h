@@ -372,7 +372,7 @@ __device__ __forceinline__ Where locate(const Params& p, int number, int R, int 
         if (x <= 0) return n;
         int c;
         if (BY_KEYS) c = x > sq.lq ? 0 : !p.causal ? (sq.lk + R - 1) / R : (min(sq.lk - 1, sq.lq - x + shift) + R) / R;
-        else c = !p.causal ? (sq.lk >= x ? n : 0) : n - (max(0, x - shift) + R - 1) / R;
+        else c = !p.causal ? (sq.lk >= x ? n : 0) : n - (max(0, min(x, sq.lk + 1) - shift) + R - 1) / R;      // (the min: 32 bits hold it)
         return max(0, min(n, c));
     };
     const int all = __builtin_amdgcn_readlane(wave_scan(n), 63);

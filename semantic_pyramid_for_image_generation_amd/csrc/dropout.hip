@@ -68,7 +68,7 @@ extern "C" int sempyr_dropout_add(int dtype, const void* x, const void* res, voi
                                   void* stream)
 {
     if (!dtype_ok(dtype)) SEMPYR_FAIL("dropout_add: unknown element type %d", dtype);
-    if (n < 0 || n > (int64_t)1 << 40) SEMPYR_FAIL("dropout_add: %lld elements", (long long)n);
+    if (n < 0 || n > (int64_t)1 << 34) SEMPYR_FAIL("dropout_add: %lld elements", (long long)n);
     if (!(p >= 0.0 && p <= 1.0)) SEMPYR_FAIL("dropout_add: p must lie in [0, 1], got %g", p);
     if (n == 0) return 0;
     if (!x || !y || !rng) SEMPYR_FAIL("dropout_add: null pointer");

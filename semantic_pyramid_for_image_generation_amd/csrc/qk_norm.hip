@@ -355,7 +355,7 @@ extern "C" int sempyr_qk_norm_rope_fwd(const sempyr_rope_desc* d, const void* xq
     const void* ptrs[] = {xq, xk, yq, yk, wq, wk};
     const Launch l = prepare(d, q, ptrs, 6);
     const int64_t blocks = (l.items * l.lanes + 255) / 256;
-    if (blocks > 0x7FFFFFFF) SEMPYR_FAIL("qk_norm_rope_fwd: too many rows");
+    if (!grid_fits(blocks, 256)) SEMPYR_FAIL("qk_norm_rope_fwd: too many rows");
     const hipStream_t st = (hipStream_t)stream;
     HbmScope scope("qk_norm_rope_kernel", 2.0 * d->tokens * (d->heads_q + d->heads_k) * d->dim * dtype_size(d->dtype), st);
     return with_dtype(d->dtype, [&](auto t) { return launch<decltype(t), false>(q, l, (unsigned)blocks, st); });

@@ -44,4 +44,6 @@ static inline int with_dtype(int dtype, F f) {
 }
 static inline bool dtype_ok(int dtype) { return dtype == SEMPYR_F32 || dtype == SEMPYR_F16 || dtype == SEMPYR_BF16; }
 static inline int dtype_size(int dtype) { return dtype == SEMPYR_F32 ? 4 : 2; }
+// a launch of `blocks` workgroups: the threads of a dimension have to stay below 2^32
+static inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0xFFFFFFFFll / threads; }
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

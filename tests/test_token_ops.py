@@ -132,7 +132,8 @@ def test_c_entries_refuse_bad_descriptors():
     n = ctypes.c_int64()
     assert L.sempyr_qk_norm_rope_bwd_scratch(ctypes.byref(d), ctypes.byref(n)) == 0 and n.value >= 2 * 16
     for args in ((7, 16, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, -1, 0.1, 16), (0, 16, 0, 16, 8, 1.5, 16), (0, 16, 0, 16, 8, -0.5, 16),
-                 (0, 0, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, 8, 0.1, 0), (0, 16, 0, 16, 8, float("nan"), 16)):
+                 (0, 0, 0, 16, 8, 0.1, 16), (0, 16, 0, 16, 8, 0.1, 0), (0, 16, 0, 16, 8, float("nan"), 16),
+                 (0, 16, 0, 16, 2 ** 34 + 1, 0.1, 16)):
         assert L.sempyr_dropout_add(*args, 0) < 0, args
     assert L.sempyr_dropout_add(0, 0, 0, 0, 0, 0.1, 0, 0) == 0             # nothing to do
 
@@ -143,7 +144,7 @@ def test_attention_c_entries_refuse():
     good = dict(total_q=8, total_k=8, q_stride_token=64, q_stride_head=16, k_stride_token=32, k_stride_head=16, v_stride_token=32,
                 v_stride_head=16, dtype=_lib.F32, heads_q=4, heads_k=2, dim=16, nseq=1, causal=1, scale=0.25)
     for change in (dict(dim=0), dict(dim=6), dict(dim=132), dict(dtype=-1), dict(heads_q=3), dict(heads_k=0), dict(nseq=-1),
-                   dict(scale=0.0), dict(scale=float("nan")), dict(total_q=-1), dict(total_k=2 ** 31), dict(k_stride_token=33),
+                   dict(scale=0.0), dict(scale=float("nan")), dict(scale=3e38), dict(total_q=-1), dict(total_k=2 ** 31), dict(k_stride_token=33),
                    dict(k_stride_token=8), dict(v_stride_token=2 ** 24), dict(q_stride_head=-16)):
         d = _lib.AttentionDesc(**{**good, **change})
         n = ctypes.c_int64()
@@ -163,3 +164,16 @@ def test_attention_c_entries_refuse():
     assert L.sempyr_attention_workspace(ctypes.byref(d), ctypes.byref(n)) == 0 and n.value > 0
     assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 10, n.value - 1, 16) < 0 and b"workspace" in L.sempyr_last_error_string()
     assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 9, 0, n.value, 16) < 0
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """More than 2^32 threads in a launch (none of these tensors would fit into memory)."""
+    from semantic_pyramid_for_image_generation_amd import _lib
+    L = _lib.lib
+    d = _lib.RopeDesc(2 ** 31, 32, 16, 16, 16, _lib.F32, 4096, 4096, 16, 1, (ctypes.c_int32 * 4)(8), 0, 1e-6)
+    assert L.sempyr_qk_norm_rope_fwd(ctypes.byref(d), *[16] * 8, 0) < 0 and b"rows" in L.sempyr_last_error_string()
+    row = 65536 * 16
+    for q, k in ((2 ** 30, 2 ** 30), (2 ** 24, 2 ** 24)):         # the one-pass kernel; the split one
+        d = _lib.AttentionDesc(q, k, row, 16, row, 16, row, 16, _lib.F32, 65536, 65536, 16, 1 if q > 2 ** 24 else 2 ** 24, 1, 0.25)
+        assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 10, 2 ** 62, 16) < 0 and b"tiles" in L.sempyr_last_error_string()
+        assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 15) < 0 and b"tiles" in L.sempyr_last_error_string()
