@@ -44,6 +44,7 @@ def _stream():
 class _NoCtx:
     """Stand-in for the autograd context when nothing is recorded."""
     needs_input_grad = (False,) * 16
+    next_functions = ()
 
     def save_for_backward(self, *tensors):
         pass
@@ -1870,9 +1871,28 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _no_second_order(what, *grads):
+_LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+
+
+def _mark_leaves(ctx):
+    """Notes, in the nodes that will take the gradients of leaves, the stream of their first use here: see _check_backward."""
+    for node, _ in ctx.next_functions:
+        if type(node) is _LeafNode:
+            node.metadata.setdefault("sempyr_stream", _stream())
+
+
+def _check_backward(what, ctx, *grads):
+    """Refuses second derivatives, and a gradient that would end the process: a leaf has one node for its gradient as long as
+    any graph of it lives, and the node belongs to the stream it was made on.  Handing it a gradient from a graph capture on
+    another stream makes that stream part of the capture, which cannot be recorded.  (Collected gradients pass no node.)"""
     if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
         raise NotImplementedError(f"{what}: second derivatives are not available")
+    if torch.cuda.is_current_stream_capturing() and not (_STASH_ON or _INPUT_GRADS_ONLY):
+        here = _stream()
+        for node, _ in ctx.next_functions:
+            if node is not None and node.metadata.get("sempyr_stream", here) != here:
+                raise _lib.SempyrError(f"{what}: a backward pass under graph capture, while a graph of the same leaves made on "
+                                       "another stream still lives: drop that one's results first, or use new leaves (detach())")
 
 
 class AxialRope:
@@ -1939,6 +1959,7 @@ class _QkNormRope(Function):
     @staticmethod
     def forward(ctx, q, k, positions, rope, wq, wk, eps, dtype):
         with _on_device(q.device):
+            _mark_leaves(ctx)
             q, k, positions = _rows(q), _rows(k), positions.contiguous()
             if wq is not None:
                 wq, wk = wq.contiguous(), wk.contiguous()
@@ -1952,7 +1973,7 @@ class _QkNormRope(Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        _no_second_order("qk_norm_rope", gq, gk)
+        _check_backward("qk_norm_rope", ctx, gq, gk)
         q, k, positions, wq, wk = ctx.saved_tensors
         rope, desc = ctx.cfg
         with _on_device(q.device):
@@ -2038,6 +2059,7 @@ class _Attention(Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, len_k, causal, scale, dtype):
         with _on_device(q.device):
+            _mark_leaves(ctx)
             rows = _attn_rows(q), _attn_rows(k), _attn_rows(v)
             q, k, v = (r[0] for r in rows)
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
@@ -2059,7 +2081,7 @@ class _Attention(Function):
 
     @staticmethod
     def backward(ctx, g):
-        _no_second_order("attention", g)
+        _check_backward("attention", ctx, g)
         q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
         with _on_device(q.device):
             g = g.contiguous()
@@ -2120,6 +2142,8 @@ def _dropout_raw(x, res, p, rng, dtype):
 class _DropoutAdd(Function):
     @staticmethod
     def forward(ctx, x, res, p, rng, dtype):
+        with _on_device(x.device):
+            _mark_leaves(ctx)
         rng = rng.contiguous()
         ctx.save_for_backward(rng)
         ctx.cfg = (p, dtype, res is not None)
@@ -2127,7 +2151,7 @@ class _DropoutAdd(Function):
 
     @staticmethod
     def backward(ctx, g):
-        _no_second_order("dropout_add", g)
+        _check_backward("dropout_add", ctx, g)
         p, dtype, has_res = ctx.cfg
         gx = _dropout_raw(g, None, p, ctx.saved_tensors[0], dtype) if ctx.needs_input_grad[0] else None
         return gx, (g if has_res else None), None, None, None

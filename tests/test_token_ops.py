@@ -177,3 +177,42 @@ def test_launches_beyond_the_grid_are_refused():
         d = _lib.AttentionDesc(q, k, row, 16, row, 16, row, 16, _lib.F32, 65536, 65536, 16, 1 if q > 2 ** 24 else 2 ** 24, 1, 0.25)
         assert L.sempyr_attention_fwd(ctypes.byref(d), *[16] * 10, 2 ** 62, 16) < 0 and b"tiles" in L.sempyr_last_error_string()
         assert L.sempyr_attention_bwd(ctypes.byref(d), *[16] * 15) < 0 and b"tiles" in L.sempyr_last_error_string()
+
+
+def test_captured_backward_of_leaves_that_another_graph_holds(ops, monkeypatch):
+    """The check, with a plain function on the CPU and the streams played by numbers."""
+    now = {'stream': 1, 'capturing': False}
+    monkeypatch.setattr(ops, '_stream', lambda: now['stream'])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: now['capturing'])
+
+    class Product(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a, b):
+            ops._mark_leaves(ctx)
+            ctx.save_for_backward(a, b)
+            return a * b
+
+        @staticmethod
+        def backward(ctx, g):
+            ops._check_backward("product", ctx, g)
+            a, b = ctx.saved_tensors
+            return g * b, g * a
+
+    w, x = torch.ones(3, requires_grad=True), torch.ones(3)
+    eager = Product.apply(w, x)
+    now.update(stream=2, capturing=True)
+    captured = Product.apply(w, x)
+    with pytest.raises(ops._lib.SempyrError, match="capture"):
+        torch.autograd.grad(captured.sum(), w)
+    with pytest.raises(ops._lib.SempyrError, match="capture"):
+        captured.sum().backward()
+    fresh = w.detach().requires_grad_()                            # a leaf of its own
+    assert torch.equal(torch.autograd.grad(Product.apply(fresh, x).sum(), fresh)[0], x)
+    inner = Product.apply(fresh, x)                                # no leaf of the other graph takes this gradient
+    assert torch.equal(torch.autograd.grad(Product.apply(inner, x).sum(), inner)[0], x)
+    del eager, captured                                            # nothing of the other graph lives
+    assert torch.equal(torch.autograd.grad(Product.apply(w, x).sum(), w)[0], x)
+    now.update(capturing=False)
+    kept = Product.apply(w, x)
+    now.update(stream=1)
+    assert torch.equal(torch.autograd.grad(Product.apply(w, x).sum(), w)[0], x) and kept is not None      # eager: any stream
