@@ -32,6 +32,7 @@ struct RopeParams {
     int64_t tokens;
     int heads[2], dim, pairs, axes, section_end[4], interleaved;
     int slice, slices;             // heads a group walks over, slices a token has
+    int lanes;                     // lanes of a group, for the kernels that do not know them at compile time
     float eps, inv_dim;
 };
 
@@ -124,21 +125,45 @@ __device__ __forceinline__ void lane_angles(const RopeParams& q, int p0, int64_t
     }
 }
 
+// Groups of `LANES` lanes, a power of two; LANES 0: of any number, `lanes`, where that fits more groups into a wave (six lanes
+// for heads of 96 in 16 bits: ten groups instead of eight).  The lanes behind the last whole group have none.
 template <int LANES>
-__device__ __forceinline__ float group_sum(float v) {
+struct Group {
+    int lanes, per_wave, lane, number;                 // number: within the workgroup
+    bool whole;
+
+    __device__ explicit Group(const RopeParams& q) {
+        const int at = threadIdx.x & 63;
+        lanes = LANES ? LANES : q.lanes;
+        per_wave = 64 / lanes;
+        lane = at % lanes;
+        number = (threadIdx.x >> 6) * per_wave + at / lanes;
+        whole = at < per_wave * lanes;
+    }
+    __device__ __forceinline__ float sum(float v) const {
+        if (LANES) {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
+            for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+            return v;
+        }
+        // pairwise into lane 0: at distance o the lanes below o are complete sums of what lies o, 2 o, .. behind them
+        const int at = threadIdx.x & 63;
+        for (int o = lanes > 32 ? 32 : lanes > 16 ? 16 : lanes > 8 ? 8 : lanes > 4 ? 4 : 2; o > 0; o >>= 1) {
+            const float t = __shfl(v, at + o, 64);
+            v += lane + o < lanes ? t : 0.f;
+        }
+        return __shfl(v, at - lane, 64);
+    }
+};
 
 template <typename T, int P, int LANES, bool VEC>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeParams q)
 {
-    const int lane = threadIdx.x % LANES;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const Group<LANES> group(q);
+    const int64_t item = (int64_t)blockIdx.x * 4 * group.per_wave + group.number;
     const int64_t token = item / q.slices;
-    if (token >= q.tokens) return;                     // whole groups leave: the shuffles below stay inside a group
-    const RowIo<T, P, VEC> io(q, lane);
+    if (!group.whole || token >= q.tokens) return;     // whole groups leave: the shuffles below stay inside a group
+    const RowIo<T, P, VEC> io(q, group.lane);
     float s[P], c[P];
     lane_angles<P>(q, io.p0, token, s, c);
     const bool norm = q.w[0] != nullptr;
@@ -153,7 +178,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeParams q)
             io.load((const T*)q.w[part], wa, wb);
 #pragma unroll
             for (int i = 0; i < P; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
-            const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), q.inv_dim, q.eps));
+            const float r = 1.f / sqrtf(fmaf(group.sum(sum), q.inv_dim, q.eps));
 #pragma unroll
             for (int i = 0; i < P; ++i) { a[i] *= r * wa[i]; b[i] *= r * wb[i]; }
         }
@@ -173,17 +198,17 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeParams q)
 template <typename T, int P, int LANES, bool VEC>
 __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeParams q)
 {
-    constexpr int GROUPS = 256 / LANES;
-    extern __shared__ float sh[];                      // [4 waves][2][dim]
-    const int lane = threadIdx.x % LANES;
-    const RowIo<T, P, VEC> io(q, lane);
+    extern __shared__ float sh[];                      // [4 waves][2][dim]; LANES 0: [groups][2][dim]
+    const Group<LANES> group(q);
+    const int groups = 4 * group.per_wave;
+    const RowIo<T, P, VEC> io(q, group.lane);
     const bool norm = q.w[0] != nullptr;
     const int total = q.heads[0] + q.heads[1];
     float ga[2][P], gb[2][P];
 #pragma unroll
     for (int i = 0; i < P; ++i) ga[0][i] = ga[1][i] = gb[0][i] = gb[1][i] = 0.f;
-    for (int64_t item = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES; item < q.tokens * q.slices;
-         item += (int64_t)gridDim.x * GROUPS) {
+    for (int64_t item = (int64_t)blockIdx.x * groups + group.number; group.whole && item < q.tokens * q.slices;
+         item += (int64_t)gridDim.x * groups) {
         const int64_t token = item / q.slices;
         float s[P], c[P];
         lane_angles<P>(q, io.p0, token, s, c);
@@ -208,8 +233,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeParams q)
                     sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
                     dot = fmaf(u[i] * wa[i], a[i], fmaf(v[i] * wb[i], b[i], dot));
                 }
-                const float r = 1.f / sqrtf(fmaf(group_sum<LANES>(sum), q.inv_dim, q.eps));
-                const float m = group_sum<LANES>(dot) * q.inv_dim * r;          // mean(g' w xhat)
+                const float r = 1.f / sqrtf(fmaf(group.sum(sum), q.inv_dim, q.eps));
+                const float m = group.sum(dot) * q.inv_dim * r;          // mean(g' w xhat)
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const float xa = a[i] * r, xb = b[i] * r;
@@ -223,25 +248,27 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(RopeParams q)
         }
     }
     if (!norm) return;
-    const int wave = threadIdx.x >> 6;
+    // what is added up next: a wave's sums, or every group's by itself
+    const int row = LANES ? threadIdx.x >> 6 : group.number, rows = LANES ? 4 : groups;
 #pragma unroll
     for (int part = 0; part < 2; ++part)
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             float u = ga[part][i], v = gb[part][i];
+            if (LANES) {
 #pragma unroll
-            for (int o = LANES; o < 64; o <<= 1) { u += __shfl_xor(u, o, 64); v += __shfl_xor(v, o, 64); }
-            if ((threadIdx.x & 63) < LANES && io.p0 + i < q.dim / 2) {
-                sh[(wave * 2 + part) * q.dim + io.elem(i, 0)] = u;
-                sh[(wave * 2 + part) * q.dim + io.elem(i, 1)] = v;
+                for (int o = LANES; o < 64; o <<= 1) { u += __shfl_xor(u, o, 64); v += __shfl_xor(v, o, 64); }
+            }
+            if (group.whole && (!LANES || (threadIdx.x & 63) < LANES) && io.p0 + i < q.dim / 2) {
+                sh[(row * 2 + part) * q.dim + io.elem(i, 0)] = u;
+                sh[(row * 2 + part) * q.dim + io.elem(i, 1)] = v;
             }
         }
     __syncthreads();
     for (int e = threadIdx.x; e < 2 * q.dim; e += 256) {
         const int part = e / q.dim, d = e - part * q.dim;
         float t = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) t += sh[(k * 2 + part) * q.dim + d];
+        for (int k = 0; k < rows; ++k) t += sh[(k * 2 + part) * q.dim + d];
         q.partials[(int64_t)blockIdx.x * 2 * q.dim + e] = t;
     }
 }
@@ -288,7 +315,8 @@ int check_desc(const sempyr_rope_desc* d, const char* who) {
     return 0;
 }
 
-struct Launch { int p, lanes; bool vec; int64_t items; };
+// lanes of a group (exact: the kernels with LANES 0), workgroups for one item (a slice of a token's heads) a group
+struct Launch { int lanes; bool vec, exact; int64_t blocks; };
 
 // Vector form where every row and both halves of a lane's pairs start on 16 bytes; element-wise loads otherwise (unaligned
 // views, rotated parts that are no multiple of a vector).
@@ -301,20 +329,23 @@ Launch prepare(const sempyr_rope_desc* d, RopeParams& q, const void* const* ptrs
     for (int k = 0; k < 4; ++k) { q.pairs += k < d->axes ? d->sections[k] : 0; q.section_end[k] = q.pairs; }
     q.xs_tok[0] = d->q_stride_token; q.xs_tok[1] = d->k_stride_token;
     q.xs_head[0] = d->q_stride_head; q.xs_head[1] = d->k_stride_head;
-    l.p = n;
     l.vec = (d->dim / 2) % n == 0 && (d->interleaved || q.pairs % n == 0);
     for (int k = 0; k < 2; ++k) l.vec = l.vec && q.xs_tok[k] * sz % 16 == 0 && q.xs_head[k] * sz % 16 == 0;
     for (int k = 0; k < nptrs; ++k) l.vec = l.vec && aligned16(ptrs[k]);
     const int need = (d->dim / 2 + n - 1) / n;
     l.lanes = 1;
     while (l.lanes < need) l.lanes *= 2;
+    l.exact = l.vec && 64 / need > 64 / l.lanes;
+    if (l.exact) l.lanes = need;
+    q.lanes = l.lanes;
     // A group walks over several heads to share the sines and cosines, as long as enough groups are left to fill the chip
     // (256 CUs x 8 waves).
     const int total = d->heads_q + d->heads_k;
     q.slice = 1;
     while (q.slice < 8 && q.slice < total && d->tokens * ceil_div(total, q.slice * 2) * l.lanes >= 64ll * 2048) q.slice *= 2;
     q.slices = ceil_div(total, q.slice);
-    l.items = d->tokens * q.slices;
+    const int groups = 4 * (64 / l.lanes);
+    l.blocks = (d->tokens * q.slices + groups - 1) / groups;
     return l;
 }
 
@@ -323,12 +354,17 @@ int launch(const RopeParams& q, const Launch& l, unsigned blocks, hipStream_t st
     constexpr int P = Vec16<T>::N;
     auto go = [&](auto lanes) {
         constexpr int LANES = decltype(lanes)::value;
-        const size_t lds = BWD ? 8 * (size_t)q.dim * sizeof(float) : 0;
-        if (BWD) l.vec ? qk_norm_rope_bwd_kernel<T, P, LANES, true><<<blocks, 256, lds, st>>>(q) : qk_norm_rope_bwd_kernel<T, P, LANES, false><<<blocks, 256, lds, st>>>(q);
+        // (exact groups: dim = 2 P lanes, at most 256 lanes: 32 KiB)
+        const size_t lds = BWD ? (LANES ? 4 : 4 * (64 / l.lanes)) * 2 * (size_t)q.dim * sizeof(float) : 0;
+        if (LANES == 0) {
+            if (BWD) qk_norm_rope_bwd_kernel<T, P, 0, true><<<blocks, 256, lds, st>>>(q);
+            else qk_norm_rope_kernel<T, P, 0, true><<<blocks, 256, 0, st>>>(q);
+        } else if (BWD) l.vec ? qk_norm_rope_bwd_kernel<T, P, LANES, true><<<blocks, 256, lds, st>>>(q) : qk_norm_rope_bwd_kernel<T, P, LANES, false><<<blocks, 256, lds, st>>>(q);
         else l.vec ? qk_norm_rope_kernel<T, P, LANES, true><<<blocks, 256, 0, st>>>(q) : qk_norm_rope_kernel<T, P, LANES, false><<<blocks, 256, 0, st>>>(q);
         SEMPYR_CHECK_LAUNCH();
         return 0;
     };
+    if (l.exact) return go(std::integral_constant<int, 0>());
     switch (l.lanes) {
         case 1: return go(std::integral_constant<int, 1>());
         case 2: return go(std::integral_constant<int, 2>());
@@ -354,7 +390,7 @@ extern "C" int sempyr_qk_norm_rope_fwd(const sempyr_rope_desc* d, const void* xq
     q.positions = positions; q.freqs = freqs;
     const void* ptrs[] = {xq, xk, yq, yk, wq, wk};
     const Launch l = prepare(d, q, ptrs, 6);
-    const int64_t blocks = (l.items * l.lanes + 255) / 256;
+    const int64_t blocks = l.blocks;
     if (!grid_fits(blocks, 256)) SEMPYR_FAIL("qk_norm_rope_fwd: too many rows");
     const hipStream_t st = (hipStream_t)stream;
     HbmScope scope("qk_norm_rope_kernel", 2.0 * d->tokens * (d->heads_q + d->heads_k) * d->dim * dtype_size(d->dtype), st);
@@ -382,7 +418,7 @@ extern "C" int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq
     q.positions = positions; q.freqs = freqs; q.partials = scratch;
     const void* ptrs[] = {xq, xk, gq, gk, dq, dk, wq, wk};
     const Launch l = prepare(d, q, ptrs, 8);
-    int64_t blocks = (l.items * l.lanes + 255) / 256;
+    int64_t blocks = l.blocks;
     if (blocks > MAX_BLOCKS) blocks = MAX_BLOCKS;
     const hipStream_t st = (hipStream_t)stream;
     return with_dtype(d->dtype, [&](auto t) {

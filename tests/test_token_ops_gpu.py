@@ -64,6 +64,15 @@ def test_qk_norm_rope(ops, dev, case, dtype, norm):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [24, 40, 48, 80, 96, 112, 144, 160, 192, 224, 288, 384])
+@pytest.mark.parametrize("tokens", [1, 11, 257])
+def test_qk_norm_rope_group_sizes(ops, dev, dim, tokens, dtype):
+    """Heads whose vectors are no power of two: groups of 3, 5, 6, 7, .. lanes, the last lanes of a wave without one."""
+    test_qk_norm_rope(ops, dev, (tokens, 3, 2, dim, (dim // 2,), False, False), dtype, True)
+    test_qk_norm_rope(ops, dev, (tokens, 1, 1, dim, (dim // 4, dim // 4), True, False), dtype, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_qk_norm_rope_strides(ops, dev, dtype):
     """Views that are not 16-byte aligned, heads before tokens, a last dimension that is not dense: equal to dense copies."""
     gen = torch.Generator().manual_seed(3)
