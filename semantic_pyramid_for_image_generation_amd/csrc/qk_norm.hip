@@ -10,12 +10,11 @@
 // 2^-64 of a turn a step).  The nearest quarter turn is split off in integers, the rest (at most 1/8 turn, rounded once to 24
 // bits) goes through the Taylor polynomials of sine and cosine (next terms below 2e-9 on +-pi/4).
 //
-// Bound by memory: x is read once and y written once (and g, dx).  A group of 2^k lanes owns a row (token, head); a lane holds
-// PAIRS pairs, that is two 16-byte vectors, in such a way that both halves of every pair lie in the same lane, in either pair
-// order -- the rotation needs no exchange, the norm k shuffles.  A group walks over a slice of the token's heads with the
+// Bound by memory: x is read once and y written once (and g, dx).  A group of lanes owns a row (token, head); a lane holds P
+// pairs, that is two 16-byte vectors, in such a way that both halves of every pair lie in the same lane, in either pair
+// order -- the rotation needs no exchange, the norm log2(lanes) shuffles.  A group walks over a slice of the token's heads with the
 // sines and cosines of its pairs in registers.  32768 tokens, 32 + 8 heads of 128, bf16, forward: 671 MB in 138 us (4.9 TB/s,
-// 94 % of a copy's rate); 16196 tokens, 16 + 4 heads of 96, fp16: forward 35 us, backward 63 + 4 us (a group of 8 lanes has
-// 2 idle at 96).
+// 94 % of a copy's rate); 16196 tokens, 16 + 4 heads of 96, fp16 (124 and 187 MB): forward 31 us, backward 50 + 4 us.
 #include "tokens.h"
 
 namespace {
@@ -295,7 +294,11 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restri
     if (row0 == 0 && col < 2 * dim) (col < dim ? dwq : dwk)[col < dim ? col : col - dim] = (T)sh[0][c];
 }
 
-constexpr int MAX_BLOCKS = 1024;                       // backward: four workgroups a CU, one row of partial sums each
+// Backward: three workgroups a CU (16-bit types: what the registers allow at once; a fourth would wait for the others' end), one
+// row of partial sums each.  Heads a group walks over at most: short slices spread the walks over the fixed number of
+// groups (16196 tokens, 16 + 4 heads of 96, fp16, backward: slices of 8 and 1024 workgroups 57 us, 8 and 768 52, 4 and 768 50);
+// forward: 32768 tokens, 32 + 8 heads of 128: 8 139 us, 4 143.
+constexpr int MAX_BLOCKS = 768, FWD_SLICE = 8, BWD_SLICE = 4;
 
 int check_desc(const sempyr_rope_desc* d, const char* who) {
     if (!d) SEMPYR_FAIL("%s: null descriptor", who);
@@ -320,7 +323,7 @@ struct Launch { int lanes; bool vec, exact; int64_t blocks; };
 
 // Vector form where every row and both halves of a lane's pairs start on 16 bytes; element-wise loads otherwise (unaligned
 // views, rotated parts that are no multiple of a vector).
-Launch prepare(const sempyr_rope_desc* d, RopeParams& q, const void* const* ptrs, int nptrs) {
+Launch prepare(const sempyr_rope_desc* d, RopeParams& q, const void* const* ptrs, int nptrs, int most) {
     Launch l;
     const int sz = dtype_size(d->dtype), n = 16 / sz;
     q.tokens = d->tokens; q.heads[0] = d->heads_q; q.heads[1] = d->heads_k;
@@ -342,8 +345,9 @@ Launch prepare(const sempyr_rope_desc* d, RopeParams& q, const void* const* ptrs
     // (256 CUs x 8 waves).
     const int total = d->heads_q + d->heads_k;
     q.slice = 1;
-    while (q.slice < 8 && q.slice < total && d->tokens * ceil_div(total, q.slice * 2) * l.lanes >= 64ll * 2048) q.slice *= 2;
+    while (q.slice < most && q.slice < total && d->tokens * ceil_div(total, q.slice * 2) * l.lanes >= 64ll * 2048) q.slice *= 2;
     q.slices = ceil_div(total, q.slice);
+    q.slice = ceil_div(total, q.slices);               // 20 heads in 7, 7 and 6, not 8, 8 and 4
     const int groups = 4 * (64 / l.lanes);
     l.blocks = (d->tokens * q.slices + groups - 1) / groups;
     return l;
@@ -356,11 +360,14 @@ int launch(const RopeParams& q, const Launch& l, unsigned blocks, hipStream_t st
         constexpr int LANES = decltype(lanes)::value;
         // (exact groups: dim = 2 P lanes, at most 256 lanes: 32 KiB)
         const size_t lds = BWD ? (LANES ? 4 : 4 * (64 / l.lanes)) * 2 * (size_t)q.dim * sizeof(float) : 0;
-        if (LANES == 0) {
-            if (BWD) qk_norm_rope_bwd_kernel<T, P, 0, true><<<blocks, 256, lds, st>>>(q);
-            else qk_norm_rope_kernel<T, P, 0, true><<<blocks, 256, 0, st>>>(q);
-        } else if (BWD) l.vec ? qk_norm_rope_bwd_kernel<T, P, LANES, true><<<blocks, 256, lds, st>>>(q) : qk_norm_rope_bwd_kernel<T, P, LANES, false><<<blocks, 256, lds, st>>>(q);
-        else l.vec ? qk_norm_rope_kernel<T, P, LANES, true><<<blocks, 256, 0, st>>>(q) : qk_norm_rope_kernel<T, P, LANES, false><<<blocks, 256, 0, st>>>(q);
+        auto run = [&](auto vec) {
+            constexpr bool VEC = decltype(vec)::value;
+            if constexpr (BWD) qk_norm_rope_bwd_kernel<T, P, LANES, VEC><<<blocks, 256, lds, st>>>(q);
+            else qk_norm_rope_kernel<T, P, LANES, VEC><<<blocks, 256, 0, st>>>(q);
+        };
+        if constexpr (LANES == 0) run(std::true_type());
+        else if (l.vec) run(std::true_type());
+        else run(std::false_type());
         SEMPYR_CHECK_LAUNCH();
         return 0;
     };
@@ -389,7 +396,7 @@ extern "C" int sempyr_qk_norm_rope_fwd(const sempyr_rope_desc* d, const void* xq
     q.x[0] = xq; q.x[1] = xk; q.y[0] = yq; q.y[1] = yk; q.w[0] = wq; q.w[1] = wk;
     q.positions = positions; q.freqs = freqs;
     const void* ptrs[] = {xq, xk, yq, yk, wq, wk};
-    const Launch l = prepare(d, q, ptrs, 6);
+    const Launch l = prepare(d, q, ptrs, 6, FWD_SLICE);
     const int64_t blocks = l.blocks;
     if (!grid_fits(blocks, 256)) SEMPYR_FAIL("qk_norm_rope_fwd: too many rows");
     const hipStream_t st = (hipStream_t)stream;
@@ -417,7 +424,7 @@ extern "C" int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq
     q.x[0] = xq; q.x[1] = xk; q.g[0] = gq; q.g[1] = gk; q.y[0] = dq; q.y[1] = dk; q.w[0] = wq; q.w[1] = wk;
     q.positions = positions; q.freqs = freqs; q.partials = scratch;
     const void* ptrs[] = {xq, xk, gq, gk, dq, dk, wq, wk};
-    const Launch l = prepare(d, q, ptrs, 8);
+    const Launch l = prepare(d, q, ptrs, 8, BWD_SLICE);
     int64_t blocks = l.blocks;
     if (blocks > MAX_BLOCKS) blocks = MAX_BLOCKS;
     const hipStream_t st = (hipStream_t)stream;
