@@ -1875,24 +1875,24 @@ _LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_
 
 
 def _mark_leaves(ctx):
-    """Notes, in the nodes that will take the gradients of leaves, the stream of their first use here: see _check_backward."""
+    """Notes, in the nodes that will take the gradients of leaves, that their first use here was on the default stream (or not):
+    see _check_backward."""
     for node, _ in ctx.next_functions:
         if type(node) is _LeafNode:
-            node.metadata.setdefault("sempyr_stream", _stream())
+            node.metadata.setdefault("sempyr_default", _stream() == 0)
 
 
 def _check_backward(what, ctx, *grads):
     """Refuses second derivatives, and a gradient that would end the process: a leaf has one node for its gradient as long as
-    any graph of it lives, and the node belongs to the stream it was made on.  Handing it a gradient from a graph capture on
-    another stream makes that stream part of the capture, which cannot be recorded.  (Collected gradients pass no node.)"""
+    any graph of it lives, and the node belongs to the stream it was made on.  Handed a gradient inside a graph capture, that
+    stream joins the capture, which the default stream cannot.  (Collected gradients pass no node.)"""
     if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
         raise NotImplementedError(f"{what}: second derivatives are not available")
     if torch.cuda.is_current_stream_capturing() and not (_STASH_ON or _INPUT_GRADS_ONLY):
-        here = _stream()
         for node, _ in ctx.next_functions:
-            if node is not None and node.metadata.get("sempyr_stream", here) != here:
+            if node is not None and node.metadata.get("sempyr_default"):
                 raise _lib.SempyrError(f"{what}: a backward pass under graph capture, while a graph of the same leaves made on "
-                                       "another stream still lives: drop that one's results first, or use new leaves (detach())")
+                                       "the default stream still lives: drop that one's results first, or use new leaves (detach())")
 
 
 class AxialRope:

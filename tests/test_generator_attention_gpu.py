@@ -190,6 +190,41 @@ def test_operators_from_one_graph(dev, dtype):
         assert all(torch.equal(a, b) for a, b in zip(out, want)), (i, bounds)
 
 
+def test_graphed_callable(dev):
+    """A training step whose forward and backward are separate graphs that torch makes from a module with the operators."""
+    from semantic_pyramid_for_image_generation_amd import ops
+
+    class Step(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.wq, self.wk = (torch.nn.Parameter(torch.rand(64) + 0.5) for _ in range(2))
+            self.register_buffer('pos', torch.arange(150, dtype=torch.int32))
+            self.register_buffer('cu', torch.tensor([0, 40, 150], dtype=torch.int32))
+            self.register_buffer('rng', torch.tensor([5, 6]))
+            self.rope = ops.AxialRope((32,))
+
+        def forward(self, x):
+            q, k, v = x[:, :4], x[:, 4:6], x[:, 6:]
+            q, k = ops.qk_norm_rope(q, k, self.pos, self.rope, self.wq, self.wk)
+            return ops.dropout_add(ops.attention(q, k, v, self.cu, causal=True), None, 0.25, self.rng)
+
+    torch.manual_seed(0)
+    eager, graphed = Step().to(dev), Step().to(dev)
+    graphed.load_state_dict(eager.state_dict())
+    graphed = torch.cuda.make_graphed_callables(graphed, (torch.randn(150, 8, 64, device=dev, requires_grad=True),))
+    for _ in range(3):
+        x, g = torch.randn(150, 8, 64, device=dev), torch.randn(150, 4, 64, device=dev)
+        results = []
+        for m in (eager, graphed):
+            m.zero_grad(set_to_none=True)
+            xi = x.clone().requires_grad_()
+            y = m(xi)
+            y.backward(g)
+            results.append([y.detach().clone(), xi.grad, m.wq.grad.clone(), m.wk.grad.clone()])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_two_graphs_and_two_streams(dev):
     """Two captured token passes (their workspaces are the graphs') replayed side by side, and eager calls on two streams: no
     state is shared."""
@@ -221,6 +256,25 @@ def test_two_graphs_and_two_streams(dev):
                 eager.append(call(x))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(eager, want))
+
+
+def test_captured_backward_beside_an_eager_graph_is_refused(dev):
+    from semantic_pyramid_for_image_generation_amd import ops
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    x = torch.randn(5, 1, 64, device=dev).requires_grad_()
+    eager = ops.attention(x, x, x, cu)
+    node = torch.autograd.graph.get_gradient_edge(x).node
+    assert ops._stream() == 0 and node.metadata['sempyr_default']          # what the check goes by
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.attention(x, x, x, cu)
+        with pytest.raises(ops._lib.SempyrError, match="capture"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, eager)
+    torch.autograd.grad(eager, x, torch.ones_like(y))
 
 
 def test_rope_table_inside_a_capture_is_refused(dev):

@@ -181,7 +181,7 @@ def test_launches_beyond_the_grid_are_refused():
 
 def test_captured_backward_of_leaves_that_another_graph_holds(ops, monkeypatch):
     """The check, with a plain function on the CPU and the streams played by numbers."""
-    now = {'stream': 1, 'capturing': False}
+    now = {'stream': 0, 'capturing': False}
     monkeypatch.setattr(ops, '_stream', lambda: now['stream'])
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: now['capturing'])
 
@@ -211,8 +211,13 @@ def test_captured_backward_of_leaves_that_another_graph_holds(ops, monkeypatch):
     inner = Product.apply(fresh, x)                                # no leaf of the other graph takes this gradient
     assert torch.equal(torch.autograd.grad(Product.apply(inner, x).sum(), inner)[0], x)
     del eager, captured                                            # nothing of the other graph lives
+    now.update(stream=1, capturing=False)
+    side = Product.apply(w, x)                                     # made on a stream that can join a capture
+    now.update(stream=2, capturing=True)
     assert torch.equal(torch.autograd.grad(Product.apply(w, x).sum(), w)[0], x)
-    now.update(capturing=False)
+    del side
+    assert torch.equal(torch.autograd.grad(Product.apply(w, x).sum(), w)[0], x)
+    now.update(stream=0, capturing=False)
     kept = Product.apply(w, x)
     now.update(stream=1)
     assert torch.equal(torch.autograd.grad(Product.apply(w, x).sum(), w)[0], x) and kept is not None      # eager: any stream
