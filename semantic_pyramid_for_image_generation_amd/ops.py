@@ -1871,6 +1871,12 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _dense16(t):
+    """t contiguous and on 16 bytes (copied only where it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 _LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
 
 
@@ -1968,15 +1974,21 @@ class _QkNormRope(Function):
             check(L.sempyr_qk_norm_rope_fwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(), rope.table(q.device).data_ptr(),
                                             _p(wq), _p(wk), yq.data_ptr(), yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
         ctx.save_for_backward(q, k, positions, wq, wk)
-        ctx.cfg = (rope, desc)
+        ctx.cfg = (rope, desc, (q.stride(), k.stride()))
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
         _check_backward("qk_norm_rope", ctx, gq, gk)
         q, k, positions, wq, wk = ctx.saved_tensors
-        rope, desc = ctx.cfg
+        rope, desc, strides = ctx.cfg
         with _on_device(q.device):
+            positions = positions.contiguous()
+            if (q.stride(), k.stride()) != strides:          # a saved-tensor hook has laid them out anew
+                q, k = _rows(q), _rows(k)
+                desc = ctypes.byref(_rope_desc(q, k, rope, desc._obj.dtype, desc._obj.eps))
+            if wq is not None:
+                wq, wk = wq.contiguous(), wk.contiguous()
             gq, gk = gq.contiguous(), gk.contiguous()
             dq, dk = torch.empty_like(gq), torch.empty_like(gk)
             dwq = dwk = scratch = None
@@ -2076,20 +2088,26 @@ class _Attention(Function):
                                          o.data_ptr(), _p(low), _p(stats), _p(ws), n, _stream()), "sempyr_attention_fwd")
         if stats is not None:
             ctx.save_for_backward(q, k, v, o, low, stats, cu_q, cu_k, len_k)
-            ctx.cfg = desc
+            ctx.cfg = (desc, (q.stride(), k.stride(), v.stride()))
         return o
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("attention", ctx, g)
         q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
+        desc, strides = ctx.cfg
         with _on_device(q.device):
-            g = g.contiguous()
-            g = g if g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
+            g, o, low = _dense16(g), _dense16(o), low if low is None else _dense16(low)
+            stats, cu_q, cu_k, len_k = (t if t is None else t.contiguous() for t in (stats, cu_q, cu_k, len_k))
+            if (q.stride(), k.stride(), v.stride()) != strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+                # a saved-tensor hook has laid them out anew
+                rows, was = (_attn_rows(q), _attn_rows(k), _attn_rows(v)), desc._obj
+                q, k, v = (r[0] for r in rows)
+                desc = ctypes.byref(_attn_desc(*rows, was.nseq, was.causal, was.scale, was.dtype))
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             delta = torch.empty_like(stats[0])
-            check(L.sempyr_attention_bwd(ctx.cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(), cu_q.data_ptr(),
-                                         cu_k.data_ptr(), _p(len_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            check(L.sempyr_attention_bwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _p(low), stats.data_ptr(), g.data_ptr(),
+                                         cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                          delta.data_ptr(), _stream()), "sempyr_attention_bwd")
         return dq, dk, dv, None, None, None, None, None, None
 

@@ -1,0 +1,90 @@
+"""What the token operators' Python side hands to the library, without a GPU: the entry points are replaced by ones that note
+their arguments, autograd around them is the real one."""
+import types
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def ops():
+    from semantic_pyramid_for_image_generation_amd import ops
+    return ops
+
+
+@pytest.fixture
+def calls(ops, monkeypatch):
+    """The C calls of a test as (entry, descriptor fields, the other arguments)."""
+    made = []
+
+    def noting(name):
+        def call(*args):
+            desc = getattr(args[0], '_obj', None)                      # byref(struct)
+            made.append((name, {f: getattr(desc, f) for f, _ in desc._fields_} if desc is not None else None, args))
+            return 0
+        return call
+
+    entries = ['sempyr_qk_norm_rope_fwd', 'sempyr_qk_norm_rope_bwd', 'sempyr_attention_fwd', 'sempyr_attention_bwd', 'sempyr_dropout_add']
+    real = ops.L
+    monkeypatch.setattr(ops, 'L', types.SimpleNamespace(**{e: noting(e) for e in entries}, sempyr_attention_workspace=real.sempyr_attention_workspace,
+                                                        sempyr_qk_norm_rope_bwd_scratch=real.sempyr_qk_norm_rope_bwd_scratch))
+
+    class Here:
+        def __init__(self, device):
+            pass
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *exc):
+            pass
+
+    monkeypatch.setattr(ops, '_on_device', Here)
+    monkeypatch.setattr(ops, '_stream', lambda: 0)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(ops, '_token_args', lambda what, names, tensors, others=(): ops._DTYPE_CODE[tensors[0].dtype])
+    return made
+
+
+def attention_of(ops, qkv):
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32)
+    return ops.attention(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:8], cu, causal=True)
+
+
+def rope_of(ops, qkv):
+    w = torch.ones(8, requires_grad=True)
+    a, b = ops.qk_norm_rope(qkv[:, :4], qkv[:, 4:6], torch.arange(6, dtype=torch.int32), ops.AxialRope((4,)), w, w)
+    return torch.cat([a, b], dim=1)
+
+
+def strides_of(desc, parts):
+    return [(desc[f'{p}_stride_token'], desc[f'{p}_stride_head']) for p in parts]
+
+
+@pytest.mark.parametrize("run,parts", [(attention_of, 'qkv'), (rope_of, 'qk')])
+def test_backward_reads_what_saved_tensor_hooks_return(ops, calls, run, parts):
+    """A hook may hand slices of a fused projection back as dense tensors, or on other addresses: the backward pass goes by the
+    strides and the alignment of what it is given, not by the forward's."""
+    qkv = torch.randn(6, 8, 8).requires_grad_()
+    dense = lambda t: t.detach().clone(memory_format=torch.contiguous_format)
+    wide = lambda t: torch.empty(2 * t.numel() + 8, dtype=t.dtype)
+
+    def spread(t):                                                     # every second element, off the 16 bytes
+        w = wide(t)[1:2 * t.numel() + 1:2].view(t.shape)
+        w.copy_(t)
+        return w
+
+    for hook, want in ((None, [(64, 8)] * 3), (dense, [(32, 8), (16, 8), (16, 8)]), (spread, [(32, 8), (16, 8), (16, 8)])):
+        calls.clear()
+        if hook is None:
+            run(ops, qkv).sum().backward()
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: hook(t.detach())):
+                run(ops, qkv).sum().backward()
+        (_, fwd, _), (_, bwd, args) = calls
+        assert strides_of(fwd, parts) == [(64, 8)] * len(parts)
+        assert strides_of(bwd, parts) == want[:len(parts)], hook
+        assert {k: v for k, v in fwd.items() if 'stride' not in k and k != 'sections'} == \
+            {k: v for k, v in bwd.items() if 'stride' not in k and k != 'sections'}
+        if parts == 'qkv':
+            assert all(a % 16 == 0 for a in args[1:6] + (args[7],))      # q, k, v, o, o_low and the gradient
