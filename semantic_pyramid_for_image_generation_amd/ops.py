@@ -1901,6 +1901,24 @@ def _check_backward(what, ctx, *grads):
                                        "the default stream still lives: drop that one's results first, or use new leaves (detach())")
 
 
+def _save(ctx, *tensors):
+    ctx.save_for_backward(*tensors)
+    ctx.kept = [None if t is None else (t.data_ptr(), t.numel()) for t in tensors]
+
+
+def _saved(what, ctx, device, kinds):
+    """The tensors that _save() kept.  A saved-tensor hook may return them elsewhere and in another layout, but not other ones:
+    the kernels would read what is not there.  `kinds`: a function that gives their shapes and types (only called where
+    something did change)."""
+    tensors = ctx.saved_tensors
+    if [None if t is None else (t.data_ptr(), t.numel()) for t in tensors] != ctx.kept:
+        for t, (shape, dtype) in zip(tensors, kinds()):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != device):
+                raise _lib.SempyrError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, kept was "
+                                       f"{dtype} {shape} on {device}")
+    return tensors
+
+
 class AxialRope:
     """Rotary position of tokens that lie on one to four axes (a text; height and width of a map; time, height and width of a
     video).  `sections[a]` pairs of a head turn with the position on axis a; pairs beyond the sections are left alone.
@@ -1973,20 +1991,23 @@ class _QkNormRope(Function):
             desc = ctypes.byref(_rope_desc(q, k, rope, dtype, eps))
             check(L.sempyr_qk_norm_rope_fwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(), rope.table(q.device).data_ptr(),
                                             _p(wq), _p(wk), yq.data_ptr(), yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
-        ctx.save_for_backward(q, k, positions, wq, wk)
+        _save(ctx, q, k, positions, wq, wk)
         ctx.cfg = (rope, desc, (q.stride(), k.stride()))
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
         _check_backward("qk_norm_rope", ctx, gq, gk)
-        q, k, positions, wq, wk = ctx.saved_tensors
         rope, desc, strides = ctx.cfg
+        was, dtype, i32 = desc._obj, gq.dtype, torch.int32
+        q, k, positions, wq, wk = _saved("qk_norm_rope", ctx, gq.device, lambda: (
+            ((was.tokens, was.heads_q, was.dim), dtype), ((was.tokens, was.heads_k, was.dim), dtype), ((was.tokens, was.axes), i32),
+            ((was.dim,), dtype), ((was.dim,), dtype)))
         with _on_device(q.device):
             positions = positions.contiguous()
             if (q.stride(), k.stride()) != strides:          # a saved-tensor hook has laid them out anew
                 q, k = _rows(q), _rows(k)
-                desc = ctypes.byref(_rope_desc(q, k, rope, desc._obj.dtype, desc._obj.eps))
+                desc = ctypes.byref(_rope_desc(q, k, rope, was.dtype, was.eps))
             if wq is not None:
                 wq, wk = wq.contiguous(), wk.contiguous()
             gq, gk = gq.contiguous(), gk.contiguous()
@@ -2087,21 +2108,26 @@ class _Attention(Function):
             check(L.sempyr_attention_fwd(desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), _p(len_k),
                                          o.data_ptr(), _p(low), _p(stats), _p(ws), n, _stream()), "sempyr_attention_fwd")
         if stats is not None:
-            ctx.save_for_backward(q, k, v, o, low, stats, cu_q, cu_k, len_k)
+            _save(ctx, q, k, v, o, low, stats, cu_q, cu_k, len_k)
             ctx.cfg = (desc, (q.stride(), k.stride(), v.stride()))
         return o
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("attention", ctx, g)
-        q, k, v, o, low, stats, cu_q, cu_k, len_k = ctx.saved_tensors
         desc, strides = ctx.cfg
+        was, dtype, i32 = desc._obj, g.dtype, torch.int32
+        rows_q, rows_k = (was.total_q, was.heads_q, was.dim), (was.total_k, was.heads_k, was.dim)
+        q, k, v, o, low, stats, cu_q, cu_k, len_k = _saved("attention", ctx, g.device, lambda: (
+            (rows_q, dtype), (rows_k, dtype), (rows_k, dtype), (rows_q, dtype), (rows_q, dtype),
+            ((2 if dtype == torch.float32 else 1, was.heads_q, was.total_q), torch.float32), ((was.nseq + 1,), i32),
+            ((was.nseq + 1,), i32), ((was.nseq,), i32)))
         with _on_device(q.device):
             g, o, low = _dense16(g), _dense16(o), low if low is None else _dense16(low)
             stats, cu_q, cu_k, len_k = (t if t is None else t.contiguous() for t in (stats, cu_q, cu_k, len_k))
             if (q.stride(), k.stride(), v.stride()) != strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
                 # a saved-tensor hook has laid them out anew
-                rows, was = (_attn_rows(q), _attn_rows(k), _attn_rows(v)), desc._obj
+                rows = _attn_rows(q), _attn_rows(k), _attn_rows(v)
                 q, k, v = (r[0] for r in rows)
                 desc = ctypes.byref(_attn_desc(*rows, was.nseq, was.causal, was.scale, was.dtype))
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
@@ -2163,15 +2189,16 @@ class _DropoutAdd(Function):
         with _on_device(x.device):
             _mark_leaves(ctx)
         rng = rng.contiguous()
-        ctx.save_for_backward(rng)
-        ctx.cfg = (p, dtype, res is not None)
+        _save(ctx, rng)
+        ctx.cfg = (p, dtype, res is not None, tuple(rng.shape))
         return _dropout_raw(x, res, p, rng, dtype)
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("dropout_add", ctx, g)
-        p, dtype, has_res = ctx.cfg
-        gx = _dropout_raw(g, None, p, ctx.saved_tensors[0], dtype) if ctx.needs_input_grad[0] else None
+        p, dtype, has_res, shape = ctx.cfg
+        rng, = _saved("dropout_add", ctx, g.device, lambda: ((shape, torch.int64),))
+        gx = _dropout_raw(g, None, p, rng.contiguous(), dtype) if ctx.needs_input_grad[0] else None
         return gx, (g if has_res else None), None, None, None
 
 

@@ -88,3 +88,24 @@ def test_backward_reads_what_saved_tensor_hooks_return(ops, calls, run, parts):
             {k: v for k, v in bwd.items() if 'stride' not in k and k != 'sections'}
         if parts == 'qkv':
             assert all(a % 16 == 0 for a in args[1:6] + (args[7],))      # q, k, v, o, o_low and the gradient
+
+
+@pytest.mark.parametrize("run", [attention_of, rope_of])
+@pytest.mark.parametrize("change", [lambda t: t.detach().double(), lambda t: t.detach()[:1], lambda t: t.detach().to('meta')])
+def test_saved_tensors_of_another_kind_are_refused(ops, calls, run, change):
+    qkv = torch.randn(6, 8, 8).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        y = run(ops, qkv)
+    with pytest.raises(ops._lib.SempyrError, match="saved"):
+        y.sum().backward()
+    assert [c[0] for c in calls if c[0].endswith('bwd')] == []
+
+
+@pytest.mark.parametrize("change", [lambda t: t.detach().int(), lambda t: t.detach()[:1], lambda t: t.detach().to('meta')])
+def test_saved_random_state_of_another_kind_is_refused(ops, calls, change):
+    x = torch.randn(6, 8).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        y = ops.dropout_add(x, None, 0.5, torch.tensor([1, 2]))
+    with pytest.raises(ops._lib.SempyrError, match="saved"):
+        y.sum().backward()
+    assert len(calls) == 1
