@@ -1986,6 +1986,8 @@ class _QkNormRope(Function):
             _mark_leaves(ctx)
             q, k, positions = _rows(q), _rows(k), positions.contiguous()
             if wq is not None:
+                # what saved_tensors returns may be a hook's copy: the parameters whose gradients may be collected
+                ctx.w_refs = [_weak(w if w.is_contiguous() else None) for w in (wq, wk)]
                 wq, wk = wq.contiguous(), wk.contiguous()
             yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
             desc = ctypes.byref(_rope_desc(q, k, rope, dtype, eps))
@@ -2023,9 +2025,9 @@ class _QkNormRope(Function):
         if _INPUT_GRADS_ONLY:
             dwq = dwk = None
         elif dwq is not None and dwq.dtype == torch.float32:
-            if _stash(wq, dwq):
+            if _stash(ctx.w_refs[0](), dwq):
                 dwq = None
-            if _stash(wk, dwk):
+            if _stash(ctx.w_refs[1](), dwk):
                 dwk = None
         return dq, dk, None, None, dwq, dwk, None, None
 

@@ -109,3 +109,17 @@ def test_saved_random_state_of_another_kind_is_refused(ops, calls, change):
     with pytest.raises(ops._lib.SempyrError, match="saved"):
         y.sum().backward()
     assert len(calls) == 1
+
+
+def test_collected_weight_gradients_reach_the_parameter_under_hooks(ops, calls, monkeypatch):
+    """async_param_grads() collects the gradient for the parameter itself, not for the copy that a hook returned."""
+    q, k = torch.randn(6, 4, 8).requires_grad_(), torch.randn(6, 2, 8).requires_grad_()
+    wq, wk = torch.ones(8, requires_grad=True), torch.ones(8, requires_grad=True)
+    monkeypatch.setattr(ops, '_STASH_ON', True)
+    monkeypatch.setattr(ops, '_current_stream_obj', lambda device: None)
+    monkeypatch.setattr(ops, '_PENDING', [])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t):
+        a, b = ops.qk_norm_rope(q, k, torch.arange(6, dtype=torch.int32), ops.AxialRope((4,)), wq, wk)
+    (a.sum() + b.sum()).backward()
+    assert len(ops._PENDING) == 2 and all(p is w for (p, *_), w in zip(ops._PENDING, (wq, wk)))
+    assert wq.grad is None and wk.grad is None
