@@ -51,6 +51,7 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
     f32x16 dk[DPAD / 32], dv[DPAD / 32];
 #pragma unroll
     for (int c = 0; c < DPAD / 32; ++c) dk[c] = dv[c] = f32x16{};
+    ColumnScale scale;
 
     // query tiles that see any of the keys; a group's steps: head g and tile t of it, counted from the
     // sequence's end
@@ -128,6 +129,16 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
             for (int i = 0; i < 16; ++i)
                 if (ki > qb + (i / 4) * 8 + half * 4 + i % 4 + shift) sc[i] = dp[i] = 0.f;
         }
+        if constexpr (NARROW<T>) {
+            scale.fit(dp, ki < sq.lk, [&](float x) {
+#pragma unroll
+                for (int c = 0; c < DPAD / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dk[c][i] *= x;
+            });
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= scale.f;
+        }
         Frag pf, df, pr, dr;
         pipelined<Frag, DPAD / 8, BATCH<T>>([&](int i) { return Tl::col(i % 2 ? qt : ot, cbase, i / 2 % (DPAD / 32), i / 2 / (DPAD / 32)); },
                                             [&](int i, Frag f) {
@@ -157,11 +168,12 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const f32x16& a = which ? dk[c] : dv[c];
-                *reinterpret_cast<f4*>(joined + (wave * 32 + (lane & 31)) * Kt::PAD + c * 32 + r * 8 + half * 4) =
-                    f4{a[r * 4], a[r * 4 + 1], a[r * 4 + 2], a[r * 4 + 3]};
+                f4 v = {a[r * 4], a[r * 4 + 1], a[r * 4 + 2], a[r * 4 + 3]};
+                if (NARROW<T> && which) v *= ldexpf(1.f, -P_BITS<T> - scale.bits);          // the groups' powers differ
+                *reinterpret_cast<f4*>(joined + (wave * 32 + (lane & 31)) * Kt::PAD + c * 32 + r * 8 + half * 4) = v;
             }
         __syncthreads();
-        const float f = which ? p.scale : 1.f;
+        const float f = which ? p.scale : ldexpf(1.f, -P_BITS<T>);
         for (int e = threadIdx.x; e < KEYS * (DPAD / 4); e += 256) {
             const int key = e / (DPAD / 4), d = e % (DPAD / 4) * 4, row = row0 + key;
             if (row >= sq.kcap || d >= p.dim) continue;
@@ -244,6 +256,7 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIM
     f32x16 acc[DPAD / 32];
 #pragma unroll
     for (int b = 0; b < DPAD / 32; ++b) acc[b] = f32x16{};
+    ColumnScale scale;
     if (tiles) {
 #pragma unroll
         for (int u = 0; u < STAGES - 1; ++u) fill(u, u);
@@ -278,6 +291,16 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIM
                 for (int i = 0; i < 16; ++i)
                     if (key0 + n * 32 + (i / 4) * 8 + half * 4 + i % 4 >= see) dp[i] = 0.f;
             }
+            if constexpr (NARROW<T>) {
+                scale.fit(dp, true, [&](float x) {
+#pragma unroll
+                    for (int c = 0; c < DPAD / 32; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[c][i] *= x;
+                });
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] *= scale.f;
+            }
             if constexpr (sizeof(T) == 4) {
                 // 32 keys are summed by themselves first, see the forward
 #pragma unroll
@@ -306,6 +329,7 @@ __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIM
     if (!present) return;
     float f = p.scale;
     if (sizeof(T) == 4) f *= p.stats[(int64_t)p.heads_q * p.total_q + stat];
+    if (NARROW<T>) f = ldexpf(f, -P_BITS<T> - scale.bits);
     T* out = (T*)p.dq + orow;
 #pragma unroll
     for (int c = 0; c < DPAD / 32; ++c)

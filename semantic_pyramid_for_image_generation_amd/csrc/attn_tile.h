@@ -79,6 +79,43 @@ __device__ __forceinline__ typename Elem<T>::Frag rest_of(const f32x16& s, const
     return r;
 }
 
+// x of the other lane half, combined: gfx950 swaps the halves in the vector unit, no LDS round trip
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// fp16 backward: P and dS in the type's normal numbers.  P, at most 1, is kept times 2^15 (the statistics carry the shift, see Stats).
+// dS has no bound of its own, and the results may fit where it does not or where it falls among the subnormals, so every column
+// (lane pair) has a power of two for it, undone in the fp32 sums: whenever a tile's largest |dS| would pass 2^15, the power falls
+// to put that at 2^7, and the sums so far follow.  What lies 2^21 below the largest so far is subnormal; its error, 2^-32 of
+// the largest, is nothing in the sum.  bf16 has the range of fp32.  (Packed batch of 16 196 tokens, 16/4 heads, causal, fp16: heads of
+// 64 dQ 158 -> 168, dK/dV 262 -> 272 us, heads of 128 278 -> 289 and 580 -> 654: a maximum and a product an element.)
+template <typename T> constexpr bool NARROW = std::is_same<T, f16>::value;
+template <typename T> constexpr int P_BITS = NARROW<T> ? 15 : 0;
+struct ColumnScale {
+    int bits = 100;                                  // no dS yet
+    float f = 0x1p100f;
+    template <typename Rescale>
+    __device__ __forceinline__ void fit(const f32x16& s, bool counts, Rescale rescale) {
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(s[i]));
+        mx = counts ? half_max(mx) : 0.f;
+        const bool moves = mx * f > 0x1p15f && mx < INFINITY;             // (infinities and NaN go through as they are)
+        if (__any(moves)) {
+            const int to = moves ? 127 + 7 - (int)(__float_as_uint(mx) >> 23) : bits;
+            rescale(ldexpf(1.f, to - bits));
+            bits = to;
+            f = ldexpf(1.f, to);
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------------------------- tiles
 template <typename T, int DPAD, int ROWS>
 struct Tile {
@@ -217,16 +254,6 @@ __device__ __forceinline__ void load_row_frags(typename Elem<T>::Frag* f, const 
     }
 }
 
-// x of the other lane half, combined: gfx950 swaps the halves in the vector unit, no LDS round trip
-__device__ __forceinline__ float half_max(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // STEPS products from fragments read from LDS, in batches: the next batch is read before this one is used, and the scheduler
 // may move neither reads nor products across (left alone, the compiler reads every fragment into the same registers right
 // before its product, which then waits for the LDS each time).
@@ -267,12 +294,12 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 }
 
 // What the forward leaves of a row's softmax.  16-bit types: lse = c m + log2(sum), from which P = exp2(c s - lse); its rounding
-// (2^-24 of about 10) is far below theirs.  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
+// (2^-24 of about 10) is far below theirs.  (fp16: lse - 15.)  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
 // exp2(c (s - m)) / sum: with lse the gradients of 1024 keys were off by 9e-7, twice what the products themselves leave.
 template <typename T> struct Stats {
     static constexpr int N = sizeof(T) == 4 ? 2 : 1;
     static __device__ __forceinline__ void store(const Params& p, int64_t at, float m, float sum) {
-        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum);      // no key: P = exp2(-infinity)
+        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum) - P_BITS<T>;   // no key: P = exp2(-infinity)
         else {
             p.stats[at] = sum == 0.f ? INFINITY : m;
             p.stats[(int64_t)p.heads_q * p.total_q + at] = sum == 0.f ? 0.f : 1.f / sum;
