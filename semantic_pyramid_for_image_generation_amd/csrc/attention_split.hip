@@ -124,14 +124,25 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
             sum += sc[i];
         }
         l += sum;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const Frag pf = frag_of<T>(sc, k), pr = rest_of<T>(sc, pf, k);
+        if constexpr (sizeof(T) == 4) {
+            // a tile's products are summed by themselves first, see attention_fwd.hip
 #pragma unroll
             for (int c = 0; c < DPAD / 32; ++c) {
-                const Frag f = Tl::col(vt, cbase, c, k);
-                acc[c] = Elem<T>::mma(f, pf, acc[c]);
-                if constexpr (sizeof(T) == 2) acc[c] = Elem<T>::mma(f, pr, acc[c]);
+                f32x16 part = f32x16{};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) part = Elem<T>::mma(Tl::col(vt, cbase, c, k), frag_of<T>(sc, k), part);
+                acc[c] += part;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const Frag pf = frag_of<T>(sc, k), pr = rest_of<T>(sc, pf, k);
+#pragma unroll
+                for (int c = 0; c < DPAD / 32; ++c) {
+                    const Frag f = Tl::col(vt, cbase, c, k);
+                    acc[c] = Elem<T>::mma(f, pf, acc[c]);
+                    acc[c] = Elem<T>::mma(f, pr, acc[c]);
+                }
             }
         }
     }
