@@ -1824,7 +1824,7 @@ def lerp_rows(real, fake, alpha):
 
 # ------------------------------------------------------------------------------------------------
 # token operators: fp32, fp16 and bf16 tensors whose last dimension has stride 1; tensors of another device than the current
-# one run there.  First derivatives only (the critic, which needs second ones, has no tokens).
+# one run there.  First derivatives only (the critic, which needs second ones, has no tokens): create_graph=True is refused.
 # ------------------------------------------------------------------------------------------------
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
@@ -1888,12 +1888,13 @@ def _mark_leaves(ctx):
             node.metadata.setdefault("sempyr_default", _stream() == 0)
 
 
-def _check_backward(what, ctx, *grads):
-    """Refuses second derivatives, and a gradient that would end the process: a leaf has one node for its gradient as long as
+def _check_backward(what, ctx, *grads, linear=False):
+    """Refuses second derivatives (create_graph=True: what the kernels return has no graph.  The gradient of a linear operator
+    depends on the cotangent only, it is refused where that has a graph), and a gradient that would end the process: a leaf has one node for its gradient as long as
     any graph of it lives, and the node belongs to the stream it was made on.  Handed a gradient inside a graph capture, that
     stream joins the capture, which the default stream cannot.  (Collected gradients pass no node.)"""
-    if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
-        raise NotImplementedError(f"{what}: second derivatives are not available")
+    if torch.is_grad_enabled() and (not linear or any(g is not None and g.requires_grad for g in grads)):
+        raise NotImplementedError(f"{what}: second derivatives (create_graph=True) are not available")
     if torch.cuda.is_current_stream_capturing() and not (_STASH_ON or _INPUT_GRADS_ONLY):
         for node, _ in ctx.next_functions:
             if node is not None and node.metadata.get("sempyr_default"):
@@ -1994,12 +1995,12 @@ class _QkNormRope(Function):
             check(L.sempyr_qk_norm_rope_fwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(), rope.table(q.device).data_ptr(),
                                             _p(wq), _p(wk), yq.data_ptr(), yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
         _save(ctx, q, k, positions, wq, wk)
-        ctx.cfg = (rope, desc, (q.stride(), k.stride()))
+        ctx.cfg, ctx.norm = (rope, desc, (q.stride(), k.stride())), wq is not None
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
-        _check_backward("qk_norm_rope", ctx, gq, gk)
+        _check_backward("qk_norm_rope", ctx, gq, gk, linear=not ctx.norm)
         rope, desc, strides = ctx.cfg
         was, dtype, i32 = desc._obj, gq.dtype, torch.int32
         q, k, positions, wq, wk = _saved("qk_norm_rope", ctx, gq.device, lambda: (
@@ -2197,7 +2198,7 @@ class _DropoutAdd(Function):
 
     @staticmethod
     def backward(ctx, g):
-        _check_backward("dropout_add", ctx, g)
+        _check_backward("dropout_add", ctx, g, linear=True)
         p, dtype, has_res, shape = ctx.cfg
         rng, = _saved("dropout_add", ctx, g.device, lambda: ((shape, torch.int64),))
         gx = _dropout_raw(g, None, p, rng.contiguous(), dtype) if ctx.needs_input_grad[0] else None

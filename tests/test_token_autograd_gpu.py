@@ -37,3 +37,15 @@ def test_saved_on_the_host(ops, dev, dtype, pin):
         torch.empty(64 * qkv.numel(), dtype=dtype, device=dev).fill_(float("nan"))       # what freed memory would hold
         grads.append(torch.autograd.grad(y, leaves, g))
     assert all(torch.equal(a, b) for a, b in zip(*grads)) and torch.isfinite(grads[0][0]).all()
+
+
+def test_second_derivatives_are_refused(ops, dev):
+    """Also with a cotangent that needs no gradient: a penalty on such a gradient must not vanish silently."""
+    x, w = torch.randn(6, 4, 64, device=dev).requires_grad_(), torch.ones(64, device=dev, requires_grad=True)
+    cu, pos = torch.tensor([0, 6], dtype=torch.int32, device=dev), torch.arange(6, dtype=torch.int32, device=dev)
+    for y in (ops.attention(x, x, x, cu), ops.qk_norm_rope(x, x, pos, ops.AxialRope((32,)), w, w)[0]):
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+    y = ops.dropout_add(x, None, 0.5, torch.tensor([1, 2], device=dev))
+    gx, = torch.autograd.grad(y.sum(), x, create_graph=True)               # linear: the gradient is a constant
+    assert torch.equal(gx, torch.where(y == 0, 0.0, 2.0))

@@ -123,3 +123,27 @@ def test_collected_weight_gradients_reach_the_parameter_under_hooks(ops, calls, 
     (a.sum() + b.sum()).backward()
     assert len(ops._PENDING) == 2 and all(p is w for (p, *_), w in zip(ops._PENDING, (wq, wk)))
     assert wq.grad is None and wk.grad is None
+
+
+@pytest.mark.parametrize("run", [attention_of, rope_of])
+def test_second_derivatives_are_refused_for_a_constant_cotangent(ops, calls, run):
+    """sum() hands the backward pass a gradient that needs none; the result depends on the inputs all the same."""
+    qkv = torch.randn(6, 8, 8).requires_grad_()
+    with pytest.raises(NotImplementedError, match="second"):
+        torch.autograd.grad(run(ops, qkv).sum(), qkv, create_graph=True)
+    with pytest.raises(NotImplementedError, match="second"):
+        run(ops, qkv).sum().backward(create_graph=True)
+    assert [c[0] for c in calls if c[0].endswith('bwd')] == []
+    torch.autograd.grad(run(ops, qkv).sum(), qkv)
+
+
+def test_linear_operators_under_create_graph(ops, calls):
+    """The dropout and the bare rotation are linear: with a constant cotangent their gradient is a constant, and right without
+    a graph; one that needs a gradient itself is refused."""
+    rope, pos = ops.AxialRope((4,)), torch.arange(6, dtype=torch.int32)
+    for run in (lambda x: ops.dropout_add(x, None, 0.5, torch.tensor([1, 2])), lambda x: ops.qk_norm_rope(x, x[:, :2], pos, rope)[0]):
+        x = torch.randn(6, 4, 8).requires_grad_()
+        gx, = torch.autograd.grad(run(x).sum(), x, create_graph=True)
+        assert gx.shape == x.shape
+        with pytest.raises(NotImplementedError, match="second"):
+            torch.autograd.grad((run(x) * x).sum(), x, create_graph=True)
