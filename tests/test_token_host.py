@@ -147,3 +147,15 @@ def test_linear_operators_under_create_graph(ops, calls):
         assert gx.shape == x.shape
         with pytest.raises(NotImplementedError, match="second"):
             torch.autograd.grad((run(x) * x).sum(), x, create_graph=True)
+
+
+def test_forward_mode_is_refused(ops, calls):
+    """A tangent must not get lost: the operators have no forward-mode derivative, with gradients recorded or not."""
+    import torch.autograd.forward_ad as fwd
+    qkv = torch.randn(6, 8, 8)
+    for mode in (torch.enable_grad, torch.no_grad):
+        for run in (attention_of, rope_of, lambda ops, x: ops.dropout_add(x, None, 0.5, torch.tensor([1, 2]))):
+            with fwd.dual_level(), mode(), pytest.raises(NotImplementedError, match="jvp"):
+                run(ops, fwd.make_dual(qkv, torch.ones_like(qkv)))
+    with fwd.dual_level(), torch.no_grad():
+        assert attention_of(ops, qkv).shape == (6, 4, 8)               # no tangent, nothing to lose
