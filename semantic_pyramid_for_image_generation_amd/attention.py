@@ -41,11 +41,13 @@ class SelfAttention2d(nn.Module):
         key = (B, H, W, device)
         hit = self._places.get(key)
         if hit is None:
-            # kept ones are made on the host: their copy has ended when it returns, so any stream may use them next
+            # kept ones are made on the host: their copy has ended when it returns, so any stream may use them next.  (Not as
+            # inference tensors, whatever the mode of the first pass: a later one saves them for its backward pass.)
             where = device if capturing else torch.device('cpu')
-            i = torch.arange(B * H * W, device=where, dtype=torch.int32)
-            hit = (torch.stack([i // W % H, i % W], dim=1).to(device, torch.int32),
-                   torch.arange(0, (B + 1) * H * W, H * W, device=where, dtype=torch.int32).to(device))
+            with torch.inference_mode(False):
+                i = torch.arange(B * H * W, device=where, dtype=torch.int32)
+                hit = (torch.stack([i // W % H, i % W], dim=1).to(device, torch.int32),
+                       torch.arange(0, (B + 1) * H * W, H * W, device=where, dtype=torch.int32).to(device))
             if not capturing:
                 self._places[key] = hit
         return hit

@@ -49,3 +49,14 @@ def test_second_derivatives_are_refused(ops, dev):
     y = ops.dropout_add(x, None, 0.5, torch.tensor([1, 2], device=dev))
     gx, = torch.autograd.grad(y.sum(), x, create_graph=True)               # linear: the gradient is a constant
     assert torch.equal(gx, torch.where(y == 0, 0.0, 2.0))
+
+
+def test_block_in_inference_mode_then_in_training(dev):
+    from semantic_pyramid_for_image_generation_amd.attention import SelfAttention2d
+    block, x = SelfAttention2d(64).to(dev), torch.randn(2, 64, 6, 5, device=dev)
+    with torch.inference_mode():
+        y = block.eval()(x)
+    z = block.train()(x)
+    assert torch.equal(y, z)
+    z.square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in block.parameters())
