@@ -1882,12 +1882,57 @@ def _dense16(t):
 _LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
 
 
+class _Seen(Exception):
+    pass
+
+
+class _ToLeaf(Function):
+    """A node in front of a leaf's, which it hands no gradient."""
+
+    @staticmethod
+    def forward(ctx, leaf):
+        return torch.zeros(())
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def _leaf_stream(node):
+    """The stream that the node taking a leaf's gradient belongs to (the one it was made on), or None where the engine cannot be
+    asked.  It is asked by a backward pass that ends at the node, before it takes anything: no work is issued, so also inside a
+    graph capture."""
+    leaf, seen = node.variable, []
+    if not leaf.is_cuda or leaf._backward_hooks:              # (a leaf's own hooks would be called)
+        return None
+
+    def look(grads):
+        seen.append(_raw_stream(leaf.device.index))
+        raise _Seen
+
+    handle = node.register_prehook(look)
+    try:
+        with torch.enable_grad():
+            _ToLeaf.apply(leaf).backward()
+    except Exception:                                          # _Seen, or what another hook of the node says to None
+        pass
+    finally:
+        handle.remove()
+    return seen[0] if seen else None
+
+
 def _mark_leaves(ctx):
-    """Notes, in the nodes that will take the gradients of leaves, that their first use here was on the default stream (or not):
-    see _check_backward."""
+    """Notes, in the nodes that will take the gradients of leaves, whether they belong to the default stream: see _check_backward.
+    Inside a graph capture that is found out; before one, where it need not be known, the current stream stands for it."""
     for node, _ in ctx.next_functions:
         if type(node) is _LeafNode:
-            node.metadata.setdefault("sempyr_default", _stream() == 0)
+            known = None
+            if "sempyr_known" not in node.metadata and torch.cuda.is_current_stream_capturing():
+                known = _leaf_stream(node)
+            if known is not None:
+                node.metadata["sempyr_known"], node.metadata["sempyr_default"] = True, known == 0
+            else:
+                node.metadata.setdefault("sempyr_default", _stream() == 0)
 
 
 def _check_backward(what, ctx, *grads, linear=False):

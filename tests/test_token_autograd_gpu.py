@@ -60,3 +60,36 @@ def test_block_in_inference_mode_then_in_training(dev):
     assert torch.equal(y, z)
     z.square().mean().backward()
     assert all(torch.isfinite(p.grad).all() for p in block.parameters())
+
+
+def test_captured_backward_beside_another_operators_graph(ops, dev):
+    """The leaf's node was made by another operator: refused where that was on the default stream, whatever stream these operators
+    met the leaf on; fine where it was on a side stream, though they met the leaf on the default one."""
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    value, grad = torch.randn(5, 1, 64, device=dev), torch.randn(5, 1, 64, device=dev)
+    side = torch.cuda.Stream(dev)
+    for stream in (torch.cuda.default_stream(dev), side):
+        x = value.clone().requires_grad_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            kept = x * 2                                               # lives on
+        torch.cuda.synchronize()
+        eager = None
+        if stream is side:
+            eager = ops.attention(x, x, x, cu)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.attention(x, x, x, cu)
+            if stream is side:
+                gx, = torch.autograd.grad(y, x, grad)
+            else:
+                with pytest.raises(ops._lib.SempyrError, match="capture"):
+                    torch.autograd.grad(y, x, grad)
+        fresh = value.clone().requires_grad_()
+        z = ops.attention(fresh, fresh, fresh, cu)
+        want, = torch.autograd.grad(z, fresh, grad)
+        for _ in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, z) and (stream is not side or torch.equal(gx, want))
+        assert kept.requires_grad and (eager is None or torch.equal(eager, z))

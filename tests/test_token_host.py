@@ -168,3 +168,60 @@ def test_block_trains_at_a_shape_first_seen_in_inference_mode():
     with torch.inference_mode():
         block._grid(2, 3, 5, torch.device('cpu'))
     assert not any(t.is_inference() for t in block._grid(2, 3, 5, torch.device('cpu')))
+
+
+def test_leaf_nodes_are_asked_for_their_stream(ops, monkeypatch):
+    """The question runs up to the node and leaves no gradient; a leaf whose hooks it would call is not asked."""
+    monkeypatch.setattr(ops, '_raw_stream', lambda index: 77)
+
+    def leaf():
+        return torch.ones(3, requires_grad=True)
+
+    class Node:                                    # the node of a leaf, which says that it lies on the GPU
+        def __init__(self, leaf):
+            self.real = torch.autograd.graph.get_gradient_edge(leaf).node
+            self.register_prehook = self.real.register_prehook
+
+        @property
+        def variable(self):
+            v = self.real.variable
+            return OnGpu(v)
+
+    class OnGpu:
+        def __init__(self, v):
+            self.v = v
+
+        is_cuda = True
+        device = torch.device('cuda', 0)
+
+        def __getattr__(self, name):
+            return getattr(self.v, name)
+
+    monkeypatch.setattr(ops._ToLeaf, 'apply', staticmethod(lambda leaf, apply=ops._ToLeaf.apply: apply(leaf.v)))
+    w = leaf()
+    assert ops._leaf_stream(Node(w)) == 77 and w.grad is None
+    (w * 2).sum().backward()
+    assert torch.equal(w.grad, torch.full((3,), 2.0))                      # the hook is gone
+    called = []
+    w = leaf()
+    w.register_hook(lambda g: called.append(g))
+    assert ops._leaf_stream(Node(w)) is None and called == []
+    assert ops._leaf_stream(torch.autograd.graph.get_gradient_edge(leaf()).node) is None      # not on a GPU
+
+
+@pytest.mark.parametrize("first", [0, 5])
+def test_captured_backward_goes_by_the_stream_of_the_leafs_node(ops, calls, monkeypatch, first):
+    """Not by the stream on which these operators met the leaf first: another operator may have made the node before."""
+    now = {'stream': 2, 'capturing': True}
+    monkeypatch.setattr(ops, '_stream', lambda: now['stream'])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: now['capturing'])
+    monkeypatch.setattr(ops, '_leaf_stream', lambda node: first)
+    qkv = torch.randn(6, 8, 8).requires_grad_()
+    other = qkv * 2                                                         # made on stream `first`, and alive
+    y = ops.dropout_add(qkv, None, 0.5, torch.tensor([1, 2]))
+    if first == 0:
+        with pytest.raises(ops._lib.SempyrError, match="capture"):
+            torch.autograd.grad(y.sum(), qkv)
+    else:
+        torch.autograd.grad(y.sum(), qkv)
+    assert other is not None
