@@ -1935,15 +1935,15 @@ def _mark_leaves(ctx):
                 node.metadata.setdefault("sempyr_default", _stream() == 0)
 
 
-def _check_backward(what, ctx, *grads, linear=False):
+def _check_backward(what, ctx, *grads, linear=False, collected=0):
     """Refuses second derivatives (create_graph=True: what the kernels return has no graph.  The gradient of a linear operator
     depends on the cotangent only, it is refused where that has a graph), and a gradient that would end the process: a leaf has one node for its gradient as long as
     any graph of it lives, and the node belongs to the stream it was made on.  Handed a gradient inside a graph capture, that
-    stream joins the capture, which the default stream cannot.  (Collected gradients pass no node.)"""
+    stream joins the capture, which the default stream cannot.  (The last `collected` inputs' nodes are handed none.)"""
     if torch.is_grad_enabled() and (not linear or any(g is not None and g.requires_grad for g in grads)):
         raise NotImplementedError(f"{what}: second derivatives (create_graph=True) are not available")
-    if torch.cuda.is_current_stream_capturing() and not (_STASH_ON or _INPUT_GRADS_ONLY):
-        for node, _ in ctx.next_functions:
+    if torch.cuda.is_current_stream_capturing():
+        for node, _ in ctx.next_functions[:len(ctx.next_functions) - collected]:
             if node is not None and node.metadata.get("sempyr_default"):
                 raise _lib.SempyrError(f"{what}: a backward pass under graph capture, while a graph of the same leaves made on "
                                        "the default stream still lives: drop that one's results first, or use new leaves (detach())")
@@ -2047,7 +2047,9 @@ class _QkNormRope(Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        _check_backward("qk_norm_rope", ctx, gq, gk, linear=not ctx.norm)
+        fp32 = gq.dtype == torch.float32
+        _check_backward("qk_norm_rope", ctx, gq, gk, linear=not ctx.norm,
+                        collected=2 if ctx.norm and (_INPUT_GRADS_ONLY or (_STASH_ON and fp32 and all(_is_leaf_param(r()) for r in ctx.w_refs))) else 0)
         rope, desc, strides = ctx.cfg
         was, dtype, i32 = desc._obj, gq.dtype, torch.int32
         q, k, positions, wq, wk = _saved("qk_norm_rope", ctx, gq.device, lambda: (
@@ -2072,7 +2074,7 @@ class _QkNormRope(Function):
                   "sempyr_qk_norm_rope_bwd")
         if _INPUT_GRADS_ONLY:
             dwq = dwk = None
-        elif dwq is not None and dwq.dtype == torch.float32:
+        elif dwq is not None and fp32:
             if _stash(ctx.w_refs[0](), dwq):
                 dwq = None
             if _stash(ctx.w_refs[1](), dwk):

@@ -225,3 +225,23 @@ def test_captured_backward_goes_by_the_stream_of_the_leafs_node(ops, calls, monk
     else:
         torch.autograd.grad(y.sum(), qkv)
     assert other is not None
+
+
+def test_collecting_parameter_gradients_does_not_hide_a_leaf_input(ops, calls, monkeypatch):
+    """Inside async_param_grads() the weights' nodes are handed nothing, the others' still are."""
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    monkeypatch.setattr(ops, '_current_stream_obj', lambda device: None)
+    monkeypatch.setattr(ops, '_PENDING', [])
+    monkeypatch.setattr(ops, '_STASH_ON', True)
+    streams = {}
+    monkeypatch.setattr(ops, '_leaf_stream', lambda node: streams[node.variable.data_ptr()])
+    q, k = torch.randn(6, 4, 8).requires_grad_(), torch.randn(6, 2, 8).requires_grad_()
+    w = torch.ones(8, requires_grad=True)
+    run = lambda: ops.qk_norm_rope(q, k, torch.arange(6, dtype=torch.int32), ops.AxialRope((4,)), w, w)[0].sum()
+    streams.update({q.data_ptr(): 3, k.data_ptr(): 3, w.data_ptr(): 0})
+    torch.autograd.grad(run(), q)
+    assert len(ops._PENDING) == 2
+    streams[k.data_ptr()] = 0
+    y = run()
+    with pytest.raises(ops._lib.SempyrError, match="capture"):
+        torch.autograd.grad(y, q)
