@@ -26,8 +26,11 @@ class SelfAttention2d(nn.Module):
         self.q_weight = nn.Parameter(torch.ones(head_dim))
         self.k_weight = nn.Parameter(torch.ones(head_dim))
         self.rope = ops.AxialRope((head_dim // 4, head_dim // 4))
-        # {seed, offset} of the dropout's generator; the offset counts the training passes
-        self.register_buffer('rng', torch.tensor([torch.initial_seed() & (2 ** 62 - 1), 0]), persistent=False)
+        # {seed, offset} of the dropout's generator; the offset counts the training passes.  The seed is what torch's generator
+        # would give next (a copy of it is asked: other layers' seeded values stay what they are), another one for every block.
+        # Like that generator's state it is no part of the state_dict: a training that goes on exactly saves and restores it.
+        state = torch.Generator().set_state(torch.get_rng_state())
+        self.register_buffer('rng', torch.tensor([int(torch.randint(0, 2 ** 62, (), generator=state, device='cpu')), 0]), persistent=False)
         self._places = {}
 
     def init_weights(self):
