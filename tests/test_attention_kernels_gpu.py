@@ -1,0 +1,133 @@
+"""Every attention kernel at every head width that it is built for, against the definition in 64 bits (token_oracle.py derives the
+tolerances); which kernels a case runs is read from the profiler."""
+import re
+
+import pytest
+import torch
+
+import token_oracle as oracle
+from test_attention_gpu import spans, table
+from test_token_ops_gpu import TYPES, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from semantic_pyramid_for_image_generation_amd import ops
+    return ops
+
+
+def kernels(run):
+    """(result, names of the attention kernels with their head width) of run()."""
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+        out = run()
+        torch.cuda.synchronize()
+    names = set()
+    for e in p.key_averages():
+        m = re.search(r"attention_(\w+?)_kernel(?:I\w*?Li(\d+)E(?:Lb([01])E)?|<[^,>]*(?:, (\d+))?(?:, (true|false))?)", e.key)
+        if m:
+            names.add((m[1], int(m[2] or m[4] or 0), {"1": True, "0": False, "true": True, "false": False, None: None}[m[3] or m[5]]))
+    return out, names
+
+
+def check(ops, dev, dtype, lq, slots, lk, behind, hq, hk, dim, causal):
+    """Forward and gradients of one call; returns the kernels that ran."""
+    gen = torch.Generator().manual_seed(sum(lq) * 7 + dim + len(lq))
+    rand = lambda *s: torch.randn(*s, generator=gen).to(dtype)
+    tq, tk = sum(lq) + behind, sum(slots) + behind
+    q, k, v, g = rand(tq, hq, dim), rand(tk, hk, dim), rand(tk, hk, dim), rand(tq, hq, dim)
+    want = oracle.attention(q, k, v, g, spans(lq, slots, lk), causal, dim ** -0.5)
+    used = torch.zeros(tk, dtype=torch.bool)
+    for _, _, k0, n in spans(lq, slots, lk):
+        used[k0:k0 + n] = True
+    k[~used], v[~used], q[sum(lq):], g[sum(lq):] = (float("nan"),) * 4              # what no sequence uses is not read
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    len_k = None if lk == slots else torch.tensor(lk, dtype=torch.int32, device=dev)
+
+    def run():
+        o = ops.attention(*leaves, table(lq, dev), table(slots, dev), len_k, causal=causal)
+        return [o.detach(), *torch.autograd.grad(o, leaves, g.to(dev))]
+
+    got, names = kernels(run)
+    for what, a, (w, e) in zip(("o", "dq", "dk", "dv"), got, want):
+        within(a, w, e, what)
+    assert not got[0][sum(lq):].any() and not got[1][sum(lq):].any() and not got[2].cpu()[~used].any() and not got[3].cpu()[~used].any()
+    return names
+
+
+def width(dim):
+    return 32 if dim <= 32 else 64 if dim <= 64 else 128
+
+
+# queries, slots, keys in use, rows behind, query heads, key heads
+LARGE = {                                            # more than 256 tiles of 128 queries, more than 8192 rows of keys
+    "ragged": ([257, 1, 0, 300, 130], [257, 1, 0, 300, 130], [257, 1, 0, 300, 130], 0, 40, 20),
+    "slots": ([129, 70, 64, 200], [200, 70, 333, 200], [190, 0, 333, 1], 5, 48, 24),
+    "grouped": ([300, 513, 31], [700, 520, 31], [700, 513, 31], 3, 64, 8),
+}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [8, 64, 80, 96, 128])
+@pytest.mark.parametrize("name", list(LARGE))
+def test_one_pass(ops, dev, name, dim, causal, dtype):
+    lq, slots, lk, behind, hq, hk = LARGE[name]
+    names = check(ops, dev, dtype, lq, slots, lk, behind, hq, hk, dim, causal)
+    w = width(dim)
+    assert {n[:2] for n in names} == {("fwd", w), ("dq", w), ("dkdv", w)}, names
+    assert all(n[2] is False for n in names if n[0] != "fwd"), names
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [24, 64, 80, 128])
+def test_split(ops, dev, dim, causal, dtype):
+    """Few tiles: keys split over workgroups, and the products of what rounding left in the 16-bit backward."""
+    names = check(ops, dev, dtype, [70, 1, 0, 130], [400, 1, 20, 130], [390, 1, 20, 130], 2, 6, 2, dim, causal)
+    w = width(dim)
+    assert {n[:2] for n in names} >= {("split", w), ("dq", w), ("dkdv", w)} and not any(n[0] == "fwd" for n in names), names
+    assert all(n[2] is (dtype != torch.float32) for n in names if n[0] in ("dq", "dkdv")), names
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("count", [62, 63, 64, 65, 200])
+@pytest.mark.parametrize("one_pass", [True, False])
+def test_many_sequences(ops, dev, count, causal, dtype, one_pass):
+    """Up to 63 sequences a lane searches each, beyond the table is searched 64 entries at a time: both sides, in the forward kernels
+    and for queries and keys in the backward ones; empty sequences, sequences without keys, longer slots, rows behind the last."""
+    gen = torch.Generator().manual_seed(count)
+    pick = lambda lo, hi: int(torch.randint(lo, hi, (), generator=gen))
+    if one_pass:
+        lq = [0 if i % 9 == 4 else pick(20, 90) if i % 7 else pick(129, 200) for i in range(count)]
+    else:
+        lq = [0 if i % 9 == 4 else 1 for i in range(count)]                   # new tokens
+    slots = [0 if i % 11 == 3 else n + pick(0, 70) for i, n in enumerate(lq)]
+    lk = [0 if i % 13 == 5 else max(0, s - pick(0, 30)) for i, s in enumerate(slots)]
+    names = check(ops, dev, dtype, lq, slots, lk, 7, 8, 8, 32, causal)
+    assert ("fwd" if one_pass else "split") in {n[0] for n in names}, names
+
+
+def test_far_cache_in_one_pass(ops, dev):
+    """The second of two cache slots begins behind 2^31 elements; enough queries for the one-pass kernel."""
+    slot, queries, gen = 2 ** 21 + 100_000, 2500, torch.Generator(device=dev).manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=dev).bfloat16()
+    near_k, near_v, q, g = rand(3000, 8, 128), rand(3000, 8, 128), rand(queries, 16, 128), rand(queries, 16, 128)
+    k, v = (torch.zeros(slot + 3000, 8, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    k[slot:], v[slot:] = near_k, near_v
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+
+    def run(k, v, cu_q, cu_k, len_k):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = ops.attention(*leaves, cu_q, cu_k, len_k, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, g)]
+
+    far, names = kernels(lambda: run(k, v, i32(0, 0, queries), i32(0, slot, slot + 3000), i32(1, 2900)))
+    near, near_names = kernels(lambda: run(near_k, near_v, i32(0, queries), i32(0, 3000), i32(2900)))
+    assert ("fwd", 128, None) in names and names == near_names
+    for a, b in zip(far[:2] + [far[2][slot:], far[3][slot:]], near):
+        assert torch.equal(a, b)                                              # the same tiles in the same order
+    assert not far[2][1:slot].any() and not far[3][1:slot].any()
