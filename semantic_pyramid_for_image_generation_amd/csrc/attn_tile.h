@@ -293,13 +293,20 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
     *reinterpret_cast<V*>(p) = V{(T)a, (T)b, (T)c, (T)d};
 }
 
+// The reference of a row (its maximum at some tile) moves only when a score passes it by REF_SLACK powers of two: until then
+// exponentials are at most 2^8, which bf16 and the fp32 sums hold, and the sums need no rescaling.  fp32: always.
+// fp16's normal numbers end at 2^-14, and what lies below may be all of the output: a key with nearly all of the weight and no
+// value, 20000 others e^-17 below it each -- off by 0.4.  There the slack is 2 and exponentials are taken times 2^13, at most 2^15.
+// (Slack 8, 4 or 2: 200.9, 200.5, 202.2 us for the packed batch with heads of 128.)
+template <typename T> constexpr float REF_SLACK = sizeof(T) == 4 ? 0.f : NARROW<T> ? 2.f : 8.f;
+template <typename T> constexpr int REF_BITS = NARROW<T> ? 13 : 0;
 // What the forward leaves of a row's softmax.  16-bit types: lse = c m + log2(sum), from which P = exp2(c s - lse); its rounding
-// (2^-24 of about 10) is far below theirs.  (fp16: lse - 15.)  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
+// (2^-24 of about 10) is far below theirs.  (fp16: lse - 15, see P_BITS.)  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
 // exp2(c (s - m)) / sum: with lse the gradients of 1024 keys were off by 9e-7, twice what the products themselves leave.
 template <typename T> struct Stats {
     static constexpr int N = sizeof(T) == 4 ? 2 : 1;
     static __device__ __forceinline__ void store(const Params& p, int64_t at, float m, float sum) {
-        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum) - P_BITS<T>;   // no key: P = exp2(-infinity)
+        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum) - (P_BITS<T> + REF_BITS<T>);   // no key: P = exp2(-infinity)
         else {
             p.stats[at] = sum == 0.f ? INFINITY : m;
             p.stats[(int64_t)p.heads_q * p.total_q + at] = sum == 0.f ? 0.f : 1.f / sum;
@@ -313,10 +320,10 @@ __device__ __forceinline__ float score_exp(float s, float c, float x) {
     return sizeof(T) == 4 ? __builtin_amdgcn_exp2f((s - x) * c) : __builtin_amdgcn_exp2f(fmaf(s, c, -x));
 }
 template <typename T>
-__device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c; }
-// The reference of a row (its maximum at some tile) moves only when a score passes it by this many powers of two: until then
-// exponentials are at most 2^8, which every type and the fp32 sums hold, and the sums need no rescaling.  fp32: always.
-template <typename T> constexpr float REF_SLACK = sizeof(T) == 4 ? 0.f : 8.f;
+__device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c - REF_BITS<T>; }
+// what the sums so far are multiplied by when the reference moves from m to `moved`
+template <typename T>
+__device__ __forceinline__ float score_move(float m, float c, float moved) { return score_exp<T>(m, c, moved + REF_BITS<T>); }
 
 // 4 consecutive elements of the output and, where it is asked for, of what their rounding left
 template <typename T>

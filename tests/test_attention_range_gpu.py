@@ -141,3 +141,29 @@ def test_zero_and_infinite_gradients(ops, dev):
     assert torch.isfinite(dq).all()
     none = torch.autograd.grad(ops.attention(*leaves, table([T], dev)), leaves, torch.zeros_like(g).to(dev))
     assert not any(t.any() for t in none)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("below", [8.0, 12.0, 17.0])
+@pytest.mark.parametrize("queries,heads", [(1, 2), (600, 64)])          # keys split; one pass
+def test_outputs_of_the_tail(ops, dev, queries, heads, below, dtype):
+    """One key takes nearly all of the weight and has no value; the output is what 20000 keys `below` it (by e^-below each) add up to.
+    Their probabilities, 1 / e^17 = 4e-8, are far below fp16's normal numbers.
+
+    The scores are exact (0 and -below, one product), so is the exponential but for the fp32 rounding of its argument (2^-24 of 25)
+    and the unit's own (2^-22); a probability is rounded by half a step h of the type, all of them alike, and the result once.  The
+    terms of both sums, of probabilities and of products, are alike, too, and may all be rounded the same way: 2^-24 for every
+    addition in a row, a tile's 64 keys and then the tiles, for products of 16 bits all keys."""
+    keys = 20000
+    q = torch.zeros(queries, heads, 32)
+    k, v = torch.zeros(keys + 1, 1, 32), torch.rand(keys + 1, 1, 32, generator=torch.Generator().manual_seed(0)) + 0.5
+    q[..., 0], k[1:, :, 0], v[0] = 1.0, -below, 0.0
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    o = ops.attention(q.to(dev), k.to(dev), v.to(dev), table([queries], dev), table([keys + 1], dev), scale=1.0)
+    w = torch.exp(torch.tensor(-below, dtype=torch.float64))
+    want = (v[1:, 0].double().sum(dim=0) * w / (1 + keys * w)).expand(queries, heads, 32)
+    h = torch.finfo(dtype).eps / 2
+    row = keys / 64 + 64
+    bound = (2 * h + 2.0 ** -24 * (25 + 4 + row + (row if dtype == torch.float32 else keys))) * want
+    worst = float(((o.double().cpu() - want).abs() / bound).max())
+    assert worst <= 1.0, worst
