@@ -439,7 +439,8 @@ int sempyr_qk_norm_rope_bwd(const sempyr_rope_desc* d, const void* xq, const voi
  * tensor like o that takes what rounding o left, so that the gradients do not carry o's rounding.  dim <= 128 and, like all strides and pointers,
  * whole 16-byte vectors; token strides up to 2^23 elements, up to 2^30 rows.  What a sequence does not use (keys behind len_k,
  * rows of other sequences) is never read.  A NaN or an infinity in a row of its own reaches, in the forward pass, the queries
- * that see it and no others; in the backward pass it may reach the gradients of its whole sequence. */
+ * that see it and no others (a score of minus infinity hides its key); in the backward pass it may reach the gradients of its whole
+ * sequence. */
 typedef struct sempyr_attention_desc {
     int64_t total_q, total_k;
     int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head, v_stride_token, v_stride_head;

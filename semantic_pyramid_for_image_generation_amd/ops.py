@@ -2197,7 +2197,7 @@ def attention(q, k, v, cu_q, cu_k=None, len_k=None, causal=False, scale=None):
     the first entry of a table is 0.  causal: the last query sees all keys, the one before it one less, and so on.  Queries
     that see no key give zeros, as do rows behind the last sequence; keys that nobody sees get zero gradients, and what lies
     in rows behind len_k[s] is never read.  A NaN or an infinity in a sequence's own keys reaches the queries that see it (in the
-    backward pass it may reach the gradients of the whole sequence).  scale None: dim ** -0.5.  dim: a multiple of 8 (fp32: 4) up to 128.
+    backward pass it may reach the gradients of the whole sequence); a score of minus infinity hides its key.  scale None: dim ** -0.5.  dim: a multiple of 8 (fp32: 4) up to 128.
     Differentiable in q, k and v; the sums of both passes have a fixed order."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2] or 0 in q.shape[1:] or 0 in k.shape[1:] or \
             q.shape[1] % k.shape[1]:
