@@ -1882,6 +1882,10 @@ def _dense16(t):
 _LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
 
 
+def _capturing():
+    return _stream() != 0 and torch.cuda.is_current_stream_capturing()          # (the default stream cannot)
+
+
 class _Seen(Exception):
     pass
 
@@ -1924,15 +1928,17 @@ def _leaf_stream(node):
 def _mark_leaves(ctx):
     """Notes, in the nodes that will take the gradients of leaves, whether they belong to the default stream: see _check_backward.
     Inside a graph capture that is found out; before one, where it need not be known, the current stream stands for it."""
+    default = capturing = None
     for node, _ in ctx.next_functions:
         if type(node) is _LeafNode:
-            known = None
-            if "sempyr_known" not in node.metadata and torch.cuda.is_current_stream_capturing():
+            if default is None:
+                default, capturing = _stream() == 0, _capturing()
+            marks = node.metadata
+            if capturing and "sempyr_known" not in marks:
                 known = _leaf_stream(node)
-            if known is not None:
-                node.metadata["sempyr_known"], node.metadata["sempyr_default"] = True, known == 0
-            else:
-                node.metadata.setdefault("sempyr_default", _stream() == 0)
+                if known is not None:
+                    marks["sempyr_known"], marks["sempyr_default"] = True, known == 0
+            marks.setdefault("sempyr_default", default)
 
 
 def _check_backward(what, ctx, *grads, linear=False, collected=0):
@@ -1942,29 +1948,39 @@ def _check_backward(what, ctx, *grads, linear=False, collected=0):
     stream joins the capture, which the default stream cannot.  (The last `collected` inputs' nodes are handed none.)"""
     if torch.is_grad_enabled() and (not linear or any(g is not None and g.requires_grad for g in grads)):
         raise NotImplementedError(f"{what}: second derivatives (create_graph=True) are not available")
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         for node, _ in ctx.next_functions[:len(ctx.next_functions) - collected]:
             if node is not None and node.metadata.get("sempyr_default"):
                 raise _lib.SempyrError(f"{what}: a backward pass under graph capture, while a graph of the same leaves made on "
                                        "the default stream still lives: drop that one's results first, or use new leaves (detach())")
 
 
+def _leaf_of(edge):
+    """The leaf that takes the gradient of an input (contiguous, so that its gradient may be collected), or None."""
+    leaf = edge[0].variable if type(edge[0]) is _LeafNode else None
+    return leaf if leaf is not None and leaf.is_contiguous() else None
+
+
+def _places(tensors):
+    return [None if t is None else (t.data_ptr(), t.numel(), t.stride()) for t in tensors]
+
+
 def _save(ctx, *tensors):
     ctx.save_for_backward(*tensors)
-    ctx.kept = [None if t is None else (t.data_ptr(), t.numel()) for t in tensors]
+    ctx.places = _places(tensors)
 
 
-def _saved(what, ctx, device, kinds):
-    """The tensors that _save() kept.  A saved-tensor hook may return them elsewhere and in another layout, but not other ones:
-    the kernels would read what is not there.  `kinds`: a function that gives their shapes and types (only called where
-    something did change)."""
+def _saved(what, ctx, g, kinds):
+    """(the tensors that _save() kept, whether any has moved).  A saved-tensor hook may return them elsewhere and in another layout,
+    but not other ones: the kernels would read what is not there.  kinds(ctx.cfg, type of g): their shapes and types."""
     tensors = ctx.saved_tensors
-    if [None if t is None else (t.data_ptr(), t.numel()) for t in tensors] != ctx.kept:
-        for t, (shape, dtype) in zip(tensors, kinds()):
-            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != device):
-                raise _lib.SempyrError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, kept was "
-                                       f"{dtype} {shape} on {device}")
-    return tensors
+    if _places(tensors) == ctx.places:
+        return tensors, False
+    for t, (shape, dtype) in zip(tensors, kinds(ctx.cfg, g.dtype)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != g.device):
+            raise _lib.SempyrError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, kept was "
+                                   f"{dtype} {shape} on {g.device}")
+    return tensors, True
 
 
 class AxialRope:
@@ -2027,6 +2043,12 @@ def _rope_scratch(dim):
     return n.value
 
 
+def _rope_kinds(cfg, dtype):
+    d = cfg[1]._obj
+    return ((d.tokens, d.heads_q, d.dim), dtype), ((d.tokens, d.heads_k, d.dim), dtype), ((d.tokens, d.axes), torch.int32), \
+        ((d.dim,), dtype), ((d.dim,), dtype)
+
+
 class _QkNormRope(Function):
     @staticmethod
     def forward(ctx, q, k, positions, rope, wq, wk, eps, dtype):
@@ -2034,34 +2056,30 @@ class _QkNormRope(Function):
             _mark_leaves(ctx)
             q, k, positions = _rows(q), _rows(k), positions.contiguous()
             if wq is not None:
-                # what saved_tensors returns may be a hook's copy: the parameters whose gradients may be collected
-                ctx.w_refs = [_weak(w if w.is_contiguous() else None) for w in (wq, wk)]
                 wq, wk = wq.contiguous(), wk.contiguous()
             yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
             desc = ctypes.byref(_rope_desc(q, k, rope, dtype, eps))
             check(L.sempyr_qk_norm_rope_fwd(desc, q.data_ptr(), k.data_ptr(), positions.data_ptr(), rope.table(q.device).data_ptr(),
                                             _p(wq), _p(wk), yq.data_ptr(), yk.data_ptr(), _stream()), "sempyr_qk_norm_rope_fwd")
-        _save(ctx, q, k, positions, wq, wk)
-        ctx.cfg, ctx.norm = (rope, desc, (q.stride(), k.stride())), wq is not None
+        if type(ctx) is not _NoCtx:
+            _save(ctx, q, k, positions, wq, wk)
+            ctx.cfg = (rope, desc, wq is not None)
         return yq, yk
 
     @staticmethod
     def backward(ctx, gq, gk):
-        fp32 = gq.dtype == torch.float32
-        _check_backward("qk_norm_rope", ctx, gq, gk, linear=not ctx.norm,
-                        collected=2 if ctx.norm and (_INPUT_GRADS_ONLY or (_STASH_ON and fp32 and all(_is_leaf_param(r()) for r in ctx.w_refs))) else 0)
-        rope, desc, strides = ctx.cfg
-        was, dtype, i32 = desc._obj, gq.dtype, torch.int32
-        q, k, positions, wq, wk = _saved("qk_norm_rope", ctx, gq.device, lambda: (
-            ((was.tokens, was.heads_q, was.dim), dtype), ((was.tokens, was.heads_k, was.dim), dtype), ((was.tokens, was.axes), i32),
-            ((was.dim,), dtype), ((was.dim,), dtype)))
+        rope, desc, norm = ctx.cfg
+        leaves = None                            # the parameters that the weights are, where their gradients are collected
+        if norm and _STASH_ON and gq.dtype == torch.float32:
+            leaves = [_leaf_of(edge) for edge in ctx.next_functions[-2:]]
+        _check_backward("qk_norm_rope", ctx, gq, gk, linear=not norm,
+                        collected=2 if norm and (_INPUT_GRADS_ONLY or (leaves and all(leaf is not None for leaf in leaves))) else 0)
+        (q, k, positions, wq, wk), moved = _saved("qk_norm_rope", ctx, gq, _rope_kinds)
         with _on_device(q.device):
-            positions = positions.contiguous()
-            if (q.stride(), k.stride()) != strides:          # a saved-tensor hook has laid them out anew
-                q, k = _rows(q), _rows(k)
-                desc = ctypes.byref(_rope_desc(q, k, rope, was.dtype, was.eps))
-            if wq is not None:
-                wq, wk = wq.contiguous(), wk.contiguous()
+            if moved:
+                q, k, positions = _rows(q), _rows(k), positions.contiguous()
+                wq, wk = (None, None) if wq is None else (wq.contiguous(), wk.contiguous())
+                desc = ctypes.byref(_rope_desc(q, k, rope, desc._obj.dtype, desc._obj.eps))
             gq, gk = gq.contiguous(), gk.contiguous()
             dq, dk = torch.empty_like(gq), torch.empty_like(gk)
             dwq = dwk = scratch = None
@@ -2074,10 +2092,10 @@ class _QkNormRope(Function):
                   "sempyr_qk_norm_rope_bwd")
         if _INPUT_GRADS_ONLY:
             dwq = dwk = None
-        elif dwq is not None and fp32:
-            if _stash(ctx.w_refs[0](), dwq):
+        elif leaves:
+            if _stash(leaves[0], dwq):
                 dwq = None
-            if _stash(ctx.w_refs[1](), dwk):
+            if _stash(leaves[1], dwk):
                 dwk = None
         return dq, dk, None, None, dwq, dwk, None, None
 
@@ -2140,6 +2158,13 @@ def _attn_workspace(total_q, total_k, heads_q, heads_k, dim, nseq, dtype):
     return n.value
 
 
+def _attn_kinds(desc, dtype):
+    d, i32 = desc._obj, torch.int32
+    q, k = ((d.total_q, d.heads_q, d.dim), dtype), ((d.total_k, d.heads_k, d.dim), dtype)
+    stats = (2 if dtype == torch.float32 else 1, d.heads_q, d.total_q), torch.float32
+    return q, k, k, q, q, stats, ((d.nseq + 1,), i32), ((d.nseq + 1,), i32), ((d.nseq,), i32)
+
+
 class _Attention(Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, len_k, causal, scale, dtype):
@@ -2161,26 +2186,21 @@ class _Attention(Function):
                                          o.data_ptr(), _p(low), _p(stats), _p(ws), n, _stream()), "sempyr_attention_fwd")
         if stats is not None:
             _save(ctx, q, k, v, o, low, stats, cu_q, cu_k, len_k)
-            ctx.cfg = (desc, (q.stride(), k.stride(), v.stride()))
+            ctx.cfg = desc
         return o
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("attention", ctx, g)
-        desc, strides = ctx.cfg
-        was, dtype, i32 = desc._obj, g.dtype, torch.int32
-        rows_q, rows_k = (was.total_q, was.heads_q, was.dim), (was.total_k, was.heads_k, was.dim)
-        q, k, v, o, low, stats, cu_q, cu_k, len_k = _saved("attention", ctx, g.device, lambda: (
-            (rows_q, dtype), (rows_k, dtype), (rows_k, dtype), (rows_q, dtype), (rows_q, dtype),
-            ((2 if dtype == torch.float32 else 1, was.heads_q, was.total_q), torch.float32), ((was.nseq + 1,), i32),
-            ((was.nseq + 1,), i32), ((was.nseq,), i32)))
+        desc = ctx.cfg
+        (q, k, v, o, low, stats, cu_q, cu_k, len_k), moved = _saved("attention", ctx, g, _attn_kinds)
         with _on_device(q.device):
-            g, o, low = _dense16(g), _dense16(o), low if low is None else _dense16(low)
-            stats, cu_q, cu_k, len_k = (t if t is None else t.contiguous() for t in (stats, cu_q, cu_k, len_k))
-            if (q.stride(), k.stride(), v.stride()) != strides or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
-                # a saved-tensor hook has laid them out anew
-                rows = _attn_rows(q), _attn_rows(k), _attn_rows(v)
+            g = _dense16(g)
+            if moved:
+                rows, was = (_attn_rows(q), _attn_rows(k), _attn_rows(v)), desc._obj
                 q, k, v = (r[0] for r in rows)
+                o, low = _dense16(o), low if low is None else _dense16(low)
+                stats, cu_q, cu_k, len_k = (t if t is None else t.contiguous() for t in (stats, cu_q, cu_k, len_k))
                 desc = ctypes.byref(_attn_desc(*rows, was.nseq, was.causal, was.scale, was.dtype))
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             delta = torch.empty_like(stats[0])
@@ -2241,15 +2261,16 @@ class _DropoutAdd(Function):
         with _on_device(x.device):
             _mark_leaves(ctx)
         rng = rng.contiguous()
-        _save(ctx, rng)
-        ctx.cfg = (p, dtype, res is not None, tuple(rng.shape))
+        if type(ctx) is not _NoCtx:
+            _save(ctx, rng)
+            ctx.cfg = (p, dtype, res is not None, rng.shape)
         return _dropout_raw(x, res, p, rng, dtype)
 
     @staticmethod
     def backward(ctx, g):
         _check_backward("dropout_add", ctx, g, linear=True)
         p, dtype, has_res, shape = ctx.cfg
-        rng, = _saved("dropout_add", ctx, g.device, lambda: ((shape, torch.int64),))
+        (rng,), _ = _saved("dropout_add", ctx, g, lambda cfg, dtype: ((tuple(shape), torch.int64),))
         gx = _dropout_raw(g, None, p, rng.contiguous(), dtype) if ctx.needs_input_grad[0] else None
         return gx, (g if has_res else None), None, None, None
 

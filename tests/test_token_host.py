@@ -229,6 +229,7 @@ def test_captured_backward_goes_by_the_stream_of_the_leafs_node(ops, calls, monk
 
 def test_collecting_parameter_gradients_does_not_hide_a_leaf_input(ops, calls, monkeypatch):
     """Inside async_param_grads() the weights' nodes are handed nothing, the others' still are."""
+    monkeypatch.setattr(ops, '_stream', lambda: 2)
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
     monkeypatch.setattr(ops, '_current_stream_obj', lambda device: None)
     monkeypatch.setattr(ops, '_PENDING', [])
