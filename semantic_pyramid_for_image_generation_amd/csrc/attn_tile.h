@@ -95,9 +95,9 @@ __device__ __forceinline__ float half_sum(float x) {
 // fp16 backward: P and dS in the type's normal numbers.  P, at most 1, is kept times 2^15 (the statistics carry the shift, see Stats).
 // dS has no bound of its own, and the results may fit where it does not or where it falls among the subnormals, so every column
 // (lane pair) has a power of two for it, undone in the fp32 sums: whenever a tile's largest |dS| would pass 2^15, the power falls
-// to put that at 2^7, and the sums so far follow.  What lies 2^21 below the largest so far is subnormal; its error, 2^-32 of
+// to put that at 2^10, and the sums so far follow.  What lies 2^24 below the largest so far is subnormal; its error, 2^-35 of
 // the largest, is nothing in the sum.  bf16 has the range of fp32.  (Packed batch of 16 196 tokens, 16/4 heads, causal, fp16: heads of
-// 64 dQ 158 -> 168, dK/dV 262 -> 272 us, heads of 128 278 -> 289 and 580 -> 654: a maximum and a product an element.)
+// 64 dQ 158 -> 168, dK/dV 262 -> 272 us, heads of 128 278 -> 289 and 580 -> 650: a maximum and a product an element.  2^7 takes the same time, 2^12 2 % more.)
 template <typename T> constexpr bool NARROW = std::is_same<T, f16>::value;
 template <typename T> constexpr int P_BITS = NARROW<T> ? 15 : 0;
 struct ColumnScale {
@@ -111,7 +111,7 @@ struct ColumnScale {
         mx = counts ? half_max(mx) : 0.f;
         const bool moves = mx * f > 0x1p15f && mx < INFINITY;             // (infinities and NaN go through as they are)
         if (__any(moves)) {
-            const int to = moves ? 127 + 7 - (int)(__float_as_uint(mx) >> 23) : bits;
+            const int to = moves ? 127 + 10 - (int)(__float_as_uint(mx) >> 23) : bits;
             rescale(ldexpf(1.f, to - bits));
             bits = to;
             f = ldexpf(1.f, to);

@@ -92,6 +92,15 @@ def test_split(ops, dev, dim, causal, dtype):
     assert all(n[2] is (dtype != torch.float32) for n in names if n[0] in ("dq", "dkdv")), names
 
 
+@pytest.mark.parametrize("dtype,dim", [(t, d) for t in TYPES for d in (4, 12, 20, 36, 40, 56, 72, 100, 104, 120, 124) if t == torch.float32 or d % 8 == 0])
+@pytest.mark.parametrize("name", ["slots", "few"])
+def test_odd_heads(ops, dev, name, dim, dtype):
+    """Heads that end inside a tile's last 16 columns, in the one-pass and in the split kernel."""
+    args = LARGE["slots"] if name == "slots" else ([3, 40], [90, 64], [33, 64], 1, 6, 3)
+    names = check(ops, dev, dtype, *args, dim, True)
+    assert ("fwd" if name == "slots" else "split", width(dim)) in {n[:2] for n in names}, names
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("count", [62, 63, 64, 65, 200])
