@@ -14,7 +14,7 @@
 // pairs, that is two 16-byte vectors, in such a way that both halves of every pair lie in the same lane, in either pair
 // order -- the rotation needs no exchange, the norm log2(lanes) shuffles.  A group walks over a slice of the token's heads with the
 // sines and cosines of its pairs in registers.  32768 tokens, 32 + 8 heads of 128, bf16, forward: 671 MB in 138 us (4.9 TB/s,
-// 94 % of a copy's rate); 16196 tokens, 16 + 4 heads of 96, fp16 (124 and 187 MB): forward 31 us, backward 50 + 4 us.
+// 94 % of a copy's rate); 16196 tokens, 16 + 4 heads of 96, fp16 (124 and 187 MB): forward 32 us, backward 51 + 4 us.
 #include "tokens.h"
 
 namespace {
