@@ -108,7 +108,7 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
         mx = half_max(mx);
         if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {
             const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
-            const float alpha = score_move<T>(m, p.scale_log2, moved);
+            const float alpha = score_move<T>(m, base, p.scale_log2, moved);
             m = top;
             base = moved;
             l *= alpha;

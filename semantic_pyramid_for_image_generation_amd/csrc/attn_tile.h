@@ -324,9 +324,11 @@ __device__ __forceinline__ float score_exp(float s, float c, float x) {
 }
 template <typename T>
 __device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c - REF_BITS<T>; }
-// what the sums so far are multiplied by when the reference moves from m to `moved`
+// what the sums so far are multiplied by when the reference moves from m (as used: `base`) to `moved`; 1 where it stays
 template <typename T>
-__device__ __forceinline__ float score_move(float m, float c, float moved) { return score_exp<T>(m, c, moved + REF_BITS<T>); }
+__device__ __forceinline__ float score_move(float m, float base, float c, float moved) {
+    return sizeof(T) == 4 ? score_exp<T>(m, c, moved) : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - moved);
+}
 
 // 4 consecutive elements of the output and, where it is asked for, of what their rounding left
 template <typename T>

@@ -167,3 +167,23 @@ def test_outputs_of_the_tail(ops, dev, queries, heads, below, dtype):
     bound = (2 * h + 2.0 ** -24 * (25 + 4 + row + (row if dtype == torch.float32 else keys))) * want
     worst = float(((o.double().cpu() - want).abs() / bound).max())
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("queries,heads", [(8, 1), (600, 64)])          # keys split; one pass
+def test_rows_beside_a_rising_one(ops, dev, queries, heads, dtype):
+    """Rows whose scores are all 12800 next to rows whose scores rise from tile to tile: the former's sums must not move with the
+    latter's reference.  V is 0 in the first half of the keys and 1 in the second: the outputs are 1/2 and 1.  Scores are exact.  In
+    16 bits the reference is a rounded product, so that all probabilities of a row are off from a power of two alike, rounded alike
+    by at most half a step h for the second product, and added unrounded; the result is rounded once.  In fp32 they are 1 (and 0)
+    and the sums exact."""
+    keys = 16384
+    q, k, v = torch.zeros(queries, heads, 32), torch.zeros(keys, 1, 32), torch.zeros(keys, 1, 32)
+    q[0::2, :, 0], q[1::2, :, 1] = 128.0, 1.0
+    k[:, 0, 0], k[:, 0, 1] = 100.0, (torch.arange(keys) // 64 * 8).float()
+    v[keys // 2:] = 1.0
+    o = ops.attention(*(t.to(dtype).to(dev) for t in (q, k, v)), table([queries], dev), table([keys], dev), scale=0.7)
+    h = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    for got, want in ((o[0::2], 0.5), (o[1::2], 1.0)):
+        worst = float((got.double() - want).abs().max())
+        assert worst <= 2 * h * want, (want, worst)
