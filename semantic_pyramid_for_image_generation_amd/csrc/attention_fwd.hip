@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DPAD>())) WAVES_PER_SIMD((fwd_wa
         float factor = 1.f;
         if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {                // (never for NaN; a row without a key: -inf > slack)
             const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
-            const float alpha = score_move<T>(m, base, p.scale_log2, moved);
+            const float alpha = score_move<T>(m, top, p.scale_log2);
             m = top;
             base = moved;
             l *= alpha;

@@ -108,7 +108,7 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
         mx = half_max(mx);
         if (__any((mx - m) * p.scale_log2 > REF_SLACK<T>)) {
             const float top = fmaxf(m, mx), moved = score_ref<T>(top, p.scale_log2);
-            const float alpha = score_move<T>(m, base, p.scale_log2, moved);
+            const float alpha = score_move<T>(m, top, p.scale_log2);
             m = top;
             base = moved;
             l *= alpha;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(128, 1) void attention_split_kernel(Params p, Split
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
         const float mw = stats[(w * 32 + c) * 2];
-        f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - top) * p.scale_log2);
+        f[w] = score_move<T>(mw, top, p.scale_log2);
         total += f[w] * stats[(w * 32 + c) * 2 + 1];
     }
     const int head = kvh * p.group + head_of(c);
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Params p, int split
     for (int s = group; s < splits; s += 8) {
         const f2 x = ml[s * rows + row];
         if (x[1] == 0.f) continue;                   // no key in this split; its partial sums were not written
-        const float f = __builtin_amdgcn_exp2f((x[0] - top) * p.scale_log2);
+        const float f = score_move<T>(x[0], top, p.scale_log2);
         total += f * x[1];
         if (d < p.dim) v += f * *reinterpret_cast<const f4*>(part_o + (s * rows + row) * p.dim + d);
     }

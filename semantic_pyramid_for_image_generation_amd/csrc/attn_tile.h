@@ -303,32 +303,40 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
 // (Slack 8, 4 or 2: 200.9, 200.5, 202.2 us for the packed batch with heads of 128.)
 template <typename T> constexpr float REF_SLACK = sizeof(T) == 4 ? 0.f : NARROW<T> ? 2.f : 8.f;
 template <typename T> constexpr int REF_BITS = NARROW<T> ? 13 : 0;
-// What the forward leaves of a row's softmax.  16-bit types: lse = c m + log2(sum), from which P = exp2(c s - lse); its rounding
-// (2^-24 of about 10) is far below theirs.  (fp16: lse - 15, see P_BITS.)  fp32: the maximum m and the reciprocal of the sum, [2][heads_q][total_q], P =
-// exp2(c (s - m)) / sum: with lse the gradients of 1024 keys were off by 9e-7, twice what the products themselves leave.
-template <typename T> struct Stats {
-    static constexpr int N = sizeof(T) == 4 ? 2 : 1;
-    static __device__ __forceinline__ void store(const Params& p, int64_t at, float m, float sum) {
-        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : m * p.scale_log2 + __log2f(sum) - (P_BITS<T> + REF_BITS<T>);   // no key: P = exp2(-infinity)
-        else {
-            p.stats[at] = sum == 0.f ? INFINITY : m;
-            p.stats[(int64_t)p.heads_q * p.total_q + at] = sum == 0.f ? 0.f : 1.f / sum;
-        }
-    }
-};
 // exponential of a score against a row's reference x (forward: c m for 16-bit types, m for fp32).  fp32 subtracts first: exact
 // next to the maximum, so that a row with one key is that key's value to the bit.
 template <typename T>
 __device__ __forceinline__ float score_exp(float s, float c, float x) {
     return sizeof(T) == 4 ? __builtin_amdgcn_exp2f((s - x) * c) : __builtin_amdgcn_exp2f(fmaf(s, c, -x));
 }
+// (Not contracted into what it is used in: everywhere the same rounded number.)
 template <typename T>
-__device__ __forceinline__ float score_ref(float m, float c) { return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c - REF_BITS<T>; }
-// what the sums so far are multiplied by when the reference moves from m (as used: `base`) to `moved`; 1 where it stays
-template <typename T>
-__device__ __forceinline__ float score_move(float m, float base, float c, float moved) {
-    return sizeof(T) == 4 ? score_exp<T>(m, c, moved) : m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - moved);
+__device__ __forceinline__ float score_ref(float m, float c) {
+#pragma clang fp contract(off)
+    return m == -INFINITY ? 0.f : sizeof(T) == 4 ? m : m * c - REF_BITS<T>;
 }
+// what sums taken with the reference m (a row's, a wave's or a workgroup's) are multiplied by to go with another one; 1 where it is
+// the same.  (16-bit types: the references as they were used, rounded.)
+template <typename T>
+__device__ __forceinline__ float score_move(float m, float to, float c) {
+#pragma clang fp contract(off)
+    if (m == -INFINITY) return 0.f;                  // (no key so far)
+    return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? (m - to) * c : score_ref<T>(m, c) - score_ref<T>(to, c));
+}
+
+// What the forward leaves of a row's softmax.  16-bit types: lse = c m + log2(sum), from which P = exp2(c s - lse); its rounding
+// (2^-24 of about 10; of scores of 10^4, fp16's half step) is far below theirs.  (fp16: lse - 15, see P_BITS.)  fp32: the maximum m and the reciprocal of the sum,
+// [2][heads_q][total_q], P = exp2(c (s - m)) / sum: with lse the gradients of 1024 keys were off by 9e-7, twice what the products themselves leave.
+template <typename T> struct Stats {
+    static constexpr int N = sizeof(T) == 4 ? 2 : 1;
+    static __device__ __forceinline__ void store(const Params& p, int64_t at, float m, float sum) {
+        if constexpr (N == 1) p.stats[at] = sum == 0.f ? INFINITY : score_ref<T>(m, p.scale_log2) + __log2f(sum) - P_BITS<T>;      // no key: P = exp2(-infinity)
+        else {
+            p.stats[at] = sum == 0.f ? INFINITY : m;
+            p.stats[(int64_t)p.heads_q * p.total_q + at] = sum == 0.f ? 0.f : 1.f / sum;
+        }
+    }
+};
 
 // 4 consecutive elements of the output and, where it is asked for, of what their rounding left
 template <typename T>

@@ -187,3 +187,22 @@ def test_rows_beside_a_rising_one(ops, dev, queries, heads, dtype):
     for got, want in ((o[0::2], 0.5), (o[1::2], 1.0)):
         worst = float((got.double() - want).abs().max())
         assert worst <= 2 * h * want, (want, worst)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("run", [32, 64])                               # other maxima in the waves of a workgroup; in its splits
+@pytest.mark.parametrize("scale", [1.051, 0.985, 1.03])
+def test_large_scores_joined_over_splits(ops, dev, run, scale, dtype):
+    """One query, scores of 100000 and 99999 (times scale) by turns of `run` keys: parts whose maxima differ are joined by the powers
+    of two that their probabilities were taken with.  Of those a rounded product of 2^17 is off by 2^-8 of a power, alike in all
+    parts.  V is 1 at the larger scores: the output is 1 / (1 + e^-scale); rounded are P and the result (h each), and scale log2(e),
+    2^-23 of it, and the unit's exponential, 2^-22."""
+    keys = 2048
+    q, k, v = torch.zeros(1, 1, 32), torch.zeros(keys, 1, 32), torch.zeros(keys, 1, 32)
+    low = torch.arange(keys) // run % 2
+    q[..., 0], q[..., 1], k[..., 0], k[:, 0, 1] = 250.0, 1.0, 400.0, -low.float()
+    v[low == 0] = 1.0
+    o = ops.attention(*(t.to(dtype).to(dev) for t in (q, k, v)), table([1], dev), table([keys], dev), scale=scale)
+    want, h = 1 / (1 + torch.exp(torch.tensor(-scale, dtype=torch.float64)).item()), torch.finfo(dtype).eps / 2
+    worst = float((o.double() - want).abs().max())
+    assert worst <= (2 * h + 2.0 ** -20) * want, (worst / want, h)
