@@ -15,7 +15,7 @@ namespace attn {
 // which is read by rows (scores, dP) and by columns (the two gradients).  At the end the groups' sums are joined in LDS.
 // 16-bit types: a ring for every wave, no barrier in the loop (packed batch of 16 196 tokens, 16/4 heads of 64, causal, bf16:
 // 213 to 227 us, in pairs 260: there the longest walk counts).  fp32: pairs, whose rings leave room for two waves a SIMD (16 x 1024
-// tokens, 2 heads of 64: 156 us, alone 170; MFMA 75 % busy).
+// tokens, 2 heads of 64: 156 to 160 us, alone 170; MFMA 75 % busy).
 template <typename T, int DPAD> struct KeyTile {
     typedef Tile<T, DPAD, 32> Tl;
     static constexpr int SHARE = sizeof(T) == 4 ? 2 : 1, GROUPS = 4 / SHARE, KEYS = 32 * SHARE, STAGES = 2;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256, (KeyTile<T, DPAD>::WAVES_SIMD)) WAVES_PER_SIMD
     }
 }
 
-// delta and dQ (packed batch of 16 196 tokens, 16/4 heads of 64, causal, bf16: 137 to 141 us; 16 x 1024 tokens, 2 heads of 64, fp32: 123,
+// delta and dQ (packed batch of 16 196 tokens, 16/4 heads of 64, causal, bf16: 133 to 141 us; 16 x 1024 tokens, 2 heads of 64, fp32: 123,
 // MFMA 70 % busy): as the forward, with dO beside Q in registers and K read by columns, too.
 template <typename T, int DPAD, bool REST>
 __global__ __launch_bounds__(256, sizeof(T) * DPAD <= 256 ? 2 : 1) WAVES_PER_SIMD((sizeof(T) * DPAD <= 256 ? 2 : 1)) void attention_dq_kernel(Params p)

@@ -6,7 +6,7 @@
 // and the output accumulator stay in registers; K and V tiles come through a ring in LDS, the next tiles' DMA runs under the
 // current tile's products.
 //
-// 16384 tokens, 16/2 heads of 128, causal, fp16: 1.16 to 1.19 ms, 945 to 924 TFLOP/s, 85 to 83 % of an 8192^3 library product's.  Bound
+// 16384 tokens, 16/2 heads of 128, causal, fp16: 1.12 to 1.19 ms, 980 to 924 TFLOP/s, 88 to 83 % of an 8192^3 library product's.  Bound
 // by the matrix and the vector pipe in turn -- counters: MFMA busy in 50 % of the cycles, the vector pipe in 57 %, LDS waits 4 % of
 // the waves' time, no bank conflicts -- at a clock that the load takes down to 1.8 GHz.  fp32 (16 x 1024 tokens, 2 heads of 64, 89
 // to 91 us): MFMA 62 % busy, one wave a SIMD.
